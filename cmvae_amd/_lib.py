@@ -35,6 +35,18 @@ class ConvGeom(ctypes.Structure):
 _PG = ctypes.POINTER(ConvGeom)
 c_int64 = ctypes.c_int64
 
+
+
+class SetAttnDesc(ctypes.Structure):
+    """struct cmvae_set_attn (include/cmvae_abi.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'B', 'Sq', 'Sk', 'H', 'Hkv', 'D', 'causal', 'residual')] + \
+               [('scale', c_float)] + [(n, c_void_p) for n in ('q', 'k', 'v', 'dO')] + \
+               [(n, c_int64 * 3) for n in ('q_stride', 'k_stride', 'v_stride', 'dO_stride')] + \
+               [(n, c_void_p) for n in ('q_len', 'k_len', 'o', 'attn', 'lse', 'delta', 'dq', 'dk', 'dv')]
+
+
+_PS = ctypes.POINTER(SetAttnDesc)
+
 # name -> (restype, argtypes); must list every symbol of include/cmvae_abi.h
 SIGNATURES = {
     'cmvae_last_error': (ctypes.c_char_p, []),
@@ -148,6 +160,9 @@ SIGNATURES = {
     'cmvae_attention_qkv_fwd': (c_int, [c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p]),
     'cmvae_attention_qkv_bwd': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p,
                                         c_void_p, c_void_p]),
+    'cmvae_set_attention_workspace_bytes': (c_size_t, [_PS, c_int]),
+    'cmvae_set_attention_fwd': (c_int, [_PS, c_void_p, c_size_t, c_void_p]),
+    'cmvae_set_attention_bwd': (c_int, [_PS, c_void_p, c_size_t, c_void_p]),
     'cmvae_adam_step_dev': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_float, c_float,
                                     c_float, c_float, c_float, c_void_p]),
     'cmvae_adam_step': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_float,

@@ -1,0 +1,907 @@
+// Set attention and its backward pass, which recomputes the probabilities: cmvae_set_attention_{fwd,bwd}.
+//
+//   s_ij = scale q_i . k_j          valid (i, j): i < q_len, j < k_len and, if causal, j <= i + k_len - q_len
+//   p_i  = softmax of s_i over its valid j (all zero if it has none),   o_i = sum_j p_ij v_j (+ q_i if residual)
+//   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i . v_j - delta_i),   delta_i = do_i . sum_j p_ij v_j
+//   dq_i = scale sum_j ds_ij k_j (+ do_i if residual),   dk_j = scale sum_i ds_ij q_i
+//
+// The G = H / Hkv query heads that share a key head are one list of R = G * Sq rows (row r = head r / Sq, position
+// r % Sq), so a tile of keys is read once for all of them and the gradients of shared heads are summed in registers, in
+// a fixed order.
+//
+// Every product is a 32 x 32 matrix instruction with the contraction's second factor in registers.  The forward and the dq
+// kernel hold 32 query rows per wave and form S^T (keys x queries): a lane then has 16 keys of ONE query, so the softmax
+// reduces inside the lane plus one exchange between the wave's halves, and the accumulator is, as it stands, the
+// second factor of the next product (o^T = V^T P^T, dq^T = K^T dS^T).  The dkv kernel holds 32 keys per wave and forms
+// S (queries x keys) for dv^T = dO^T P and dk^T = Q^T dS.  No probability is ever stored.
+//
+// Element types: fp32 on v_mfma_f32_32x32x2_f32, bf16 / fp16 on the 32x32x16 forms.  Scores, softmax statistics,
+// delta and every accumulator are fp32; in the 16-bit types P and dS are rounded once (to nearest) to be factors.
+#include "common.h"
+
+#include <cmath>
+#include <type_traits>
+
+namespace cmvae {
+namespace sa {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+    const char *q, *k, *v, *doo, *att;
+    char *o, *ocopy, *dq, *dk, *dv;
+    float *lse, *delta, *part, *part_ml;
+    const int *q_len, *k_len;
+    long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, g_sb, g_ss, g_sh;   // strides in elements
+    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, split_tiles, ntiles;
+    float scale, c;                                                                // c = scale * log2(e)
+};
+
+// fp16 probabilities are held times 2^15 as factors: p <= 1 fits (32768 < 65504), and a row of many keys, whose p are
+// under fp16's smallest normal 2^-14, keeps 11 bits of each.  The other types have fp32's exponents.
+template <typename T> __device__ constexpr float p_shift() { return std::is_same<T, _Float16>::value ? 15.f : 0.f; }
+
+template <typename T>
+struct Vec8 {};
+template <> struct Vec8<__bf16> { typedef bf16x8 type; };
+template <> struct Vec8<_Float16> { typedef f16x8 type; };
+
+// Second factor of a product over D channels, 32 columns: D / 2 values per lane.
+template <typename T, int D>
+struct Frag {
+    u32x4 x[D * sizeof(T) / 32];
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma16(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (std::is_same<T, __bf16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// 2^x, results under 2^-126 as 0 (a weight that small adds nothing to a sum that holds a 1)
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the value of the lane 32 places away
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// row of accumulator register r in a 32 x 32 tile, for lane half h
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// The LDS pitch of a tile row: 16 bytes more than the row, so that the 32 rows of a fragment read start in different banks.
+template <typename T, int D> __host__ __device__ constexpr int pitch() { return D * (int)sizeof(T) + 16; }
+
+// ---- first factor = 32 rows of an LDS tile, contraction over the D channels -------------------------------------------
+// The contraction's order is free as long as both factors agree: lane half h takes channels 8c + 4h .. + 3 of fp32
+// (16c + 8h .. + 7 of 16-bit) rows, one 16-byte read.
+template <typename T, int D>
+__device__ __forceinline__ f32x16 mul_rows(const char* tile, int row0, const Frag<T, D>& b, f32x16 acc) {
+    const int lane = threadIdx.x & 63;
+    const char* p = tile + (row0 + (lane & 31)) * pitch<T, D>() + (lane >> 5) * 16;
+    constexpr int NC = D * sizeof(T) / 32;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(p + c * 32);
+        if constexpr (std::is_same<T, float>::value) {
+            const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b.x[c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], acc, 0, 0, 0);
+        } else {
+            acc = mma16<T>(a, b.x[c], acc);
+        }
+    }
+    return acc;
+}
+
+// ---- first factor = 32 channels x 32 rows of an LDS tile (transposed), second factor = a 32 x 32 accumulator --------
+// Register r of the accumulator is tile row acc_row(r, h), which fixes the contraction's order.  fp32: one value per
+// lane and instruction.  16-bit: registers 8s .. 8s + 7 are one instruction's eight; the matching first factor — four
+// rows at one channel, twice — comes from the transposing LDS read (16 lanes name 4 rows x 16 channels, lane i
+// receives channel i of the four rows).
+template <typename T, int D>
+__device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, f32x16 (&acc)[D / 32]) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const char* p = tile + (row0 + acc_row(r, h)) * pitch<T, D>() + (lane & 31) * 4;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(p + d * 128), w[r], acc[d], 0, 0, 0);
+        }
+    } else {
+        typedef typename Vec8<T>::type V8;
+        const int i = lane & 15;
+        const char* p = tile + (row0 + 4 * h + (i >> 2)) * pitch<T, D>() + (lane & 16) * 2 + (i & 3) * 8;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            V8 b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (T)w[8 * s + j];
+            const u32x4 bu = __builtin_bit_cast(u32x4, b);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const char* a = p + 16 * s * pitch<T, D>() + d * 64;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)(a + 8 * pitch<T, D>()));
+                const s16x8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[d] = mma16<T>(__builtin_bit_cast(u32x4, av), bu, acc[d]);
+            }
+        }
+    }
+}
+
+// one row as a second factor (lane & 31 = column); rows that are not there are zero
+template <typename T, int D>
+__device__ __forceinline__ Frag<T, D> load_frag(const char* row, bool there) {
+    const int h = (threadIdx.x & 63) >> 5;
+    Frag<T, D> f;
+#pragma unroll
+    for (int c = 0; c < (int)(D * sizeof(T) / 32); ++c) {
+        f.x[c] = u32x4{0, 0, 0, 0};
+        if (there) f.x[c] = *reinterpret_cast<const u32x4*>(row + c * 32 + h * 16);
+    }
+    return f;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ float dot_frag(const Frag<T, D>& a, const Frag<T, D>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < (int)(D * sizeof(T) / 32); ++c) {
+        if constexpr (std::is_same<T, float>::value) {
+            const f32x4 x = __builtin_bit_cast(f32x4, a.x[c]), y = __builtin_bit_cast(f32x4, b.x[c]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
+        } else {
+            typedef typename Vec8<T>::type V8;
+            const V8 x = __builtin_bit_cast(V8, a.x[c]), y = __builtin_bit_cast(V8, b.x[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
+        }
+    }
+    return s + other_half(s);
+}
+
+// four channels of a row, fp32 -> T
+template <typename T>
+__device__ __forceinline__ void store4(char* p, float a, float b, float c, float d) {
+    if constexpr (std::is_same<T, float>::value) {
+        *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+    } else {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 v = {(T)a, (T)b, (T)c, (T)d};
+        *reinterpret_cast<T4*>(p) = v;
+    }
+}
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const char* p) {
+    if constexpr (std::is_same<T, float>::value) {
+        return *reinterpret_cast<const f32x4*>(p);
+    } else {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T4 v = *reinterpret_cast<const T4*>(p);
+        return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    }
+}
+
+// ---- tiles of ROWS rows through registers into LDS: requested while the previous tile is used -----------------------
+template <typename T, int D, int ROWS, int THREADS>
+struct Stage {
+    static constexpr int CPR = D * sizeof(T) / 16;               // 16-byte pieces per row
+    static constexpr int N = ROWS * CPR / THREADS;
+    static_assert(ROWS * CPR % THREADS == 0, "whole pieces per thread");
+    u32x4 x[N];
+    // keys: consecutive rows of one tensor; rows from `end` on are zeros
+    __device__ __forceinline__ void load(const char* base, long stride_bytes, int row0, int end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * THREADS + threadIdx.x, row = row0 + id / CPR;
+            x[i] = u32x4{0, 0, 0, 0};
+            if (row < end) x[i] = *reinterpret_cast<const u32x4*>(base + row * stride_bytes + (id % CPR) * 16);
+        }
+    }
+    // query rows r0 .. of a key head's list: (head, position) = divmod(r, Sq); positions from q_end on are zeros
+    __device__ __forceinline__ void load_rows(const char* base, long ss, long sh, int r0, int R, int Sq, int q_end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * THREADS + threadIdx.x, r = r0 + id / CPR;
+            x[i] = u32x4{0, 0, 0, 0};
+            if (r < R) {
+                const int g = r / Sq, pos = r - g * Sq;
+                if (pos < q_end) x[i] = *reinterpret_cast<const u32x4*>(base + pos * ss + g * sh + (id % CPR) * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = i * THREADS + threadIdx.x;
+            *reinterpret_cast<u32x4*>(tile + (id / CPR) * pitch<T, D>() + (id % CPR) * 16) = x[i];
+        }
+    }
+};
+
+struct Place {           // what a workgroup works on
+    int b, kh, tile, split;
+};
+// (batch, key head) runs fastest: with a multiple of 8 of them each stays on one XCD, whose L2 then holds its keys
+__device__ __forceinline__ Place place(const Args& a, bool last_first) {
+    const int nbh = a.B * a.Hkv;
+    int id = blockIdx.x;
+    Place p;
+    const int bh = id % nbh;
+    id /= nbh;
+    p.split = id % a.nsplit;
+    id /= a.nsplit;
+    p.tile = last_first ? a.ntiles - 1 - id : id;
+    p.b = bh / a.Hkv;
+    p.kh = bh - p.b * a.Hkv;
+    return p;
+}
+
+__device__ __forceinline__ void lens(const Args& a, int b, int& ql, int& kl) {
+    ql = a.Sq;
+    kl = a.Sk;
+    if (a.q_len) ql = min(max(a.q_len[b], 0), a.Sq);
+    if (a.k_len) kl = min(max(a.k_len[b], 0), a.Sk);
+}
+
+// positions [lo, hi] that the rows r0 .. r1 - 1 of a key head's list cover
+__device__ __forceinline__ void span(const Args& a, int r0, int r1, int& lo, int& hi) {
+    const int g0 = r0 / a.Sq, g1 = (r1 - 1) / a.Sq;
+    if (g0 == g1) {
+        lo = r0 - g0 * a.Sq;
+        hi = r1 - 1 - g0 * a.Sq;
+    } else {
+        lo = 0;
+        hi = a.Sq - 1;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// NW waves of 32 rows; keys in tiles of KT through LDS, two buffers.  Running maximum m (log2 units) and sum l per row.
+// nsplit > 1: a workgroup covers split_tiles tiles and leaves (acc, m, l) for the joining kernel.
+template <typename T, int D, int NW, int KT>
+__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int TB = KT * pitch<T, D>();
+    const Place pl = place(a, a.causal);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+    int ql, kl;
+    lens(a, pl.b, ql, kl);
+    const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
+    const int g = r / a.Sq, pos = r - g * a.Sq;
+    const bool row_ok = r < a.R && pos < ql;
+    const int off = kl - ql;
+    int lo, hi, kend = kl;
+    span(a, r0, min(r0 + NW * 32, a.R), lo, hi);
+    if (a.causal) kend = min(kl, min(hi, ql - 1) + off + 1);
+    if (lo >= ql) kend = 0;
+    int t0 = 0, t1 = (max(kend, 0) + KT - 1) / KT;
+    if (a.nsplit > 1) {
+        t0 = pl.split * a.split_tiles;
+        t1 = min(t1, t0 + a.split_tiles);
+    }
+    const long es = sizeof(T);
+    const char* kb = a.k + (pl.b * a.k_sb + pl.kh * a.k_sh) * es;
+    const char* vb = a.v + (pl.b * a.v_sb + pl.kh * a.v_sh) * es;
+    const char* qrow = a.q + (pl.b * a.q_sb + pos * a.q_ss + (pl.kh * a.G + g) * a.q_sh) * es;
+    const Frag<T, D> qf = load_frag<T, D>(qrow, row_ok);
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) acc[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+    const int klast = a.causal ? min(kl, pos + off + 1) : kl;      // this row's keys end here
+
+    Stage<T, D, KT, NW * 64> ks, vs;
+    if (t0 < t1) {
+        ks.load(kb, a.k_ss * es, t0 * KT, kl);
+        vs.load(vb, a.v_ss * es, t0 * KT, kl);
+        ks.put(smem);
+        vs.put(smem + TB);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const char* kt = smem + ((t - t0) & 1) * 2 * TB;
+        const char* vt = kt + TB;
+        if (t + 1 < t1) {
+            ks.load(kb, a.k_ss * es, (t + 1) * KT, kl);
+            vs.load(vb, a.v_ss * es, (t + 1) * KT, kl);
+        }
+        f32x16 s[KT / 32];
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) s[u] = mul_rows<T, D>(kt, u * 32, qf, zero16());
+        const int k0 = t * KT;
+        if (k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1)) {
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + u * 32 + acc_row(i, h) >= klast) s[u][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+        mx = fmaxf(mx, other_half(mx));
+        const float mn = fmaxf(m, mx * a.c);
+        const float mu = mn == -INFINITY ? 0.f : mn;               // a row without a valid key so far: every p is 0
+        const float al = exp2_raw(m - mu), sub = mu - p_shift<T>();
+        m = mn;
+        float ps = 0.f;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = exp2_raw(fmaf(s[u][i], a.c, -sub));
+                ps += s[u][i];
+            }
+        l = fmaf(l, al, ps);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= al;
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) mul_cols<T, D>(vt, u * 32, s[u], acc);
+        if (t + 1 < t1) {
+            char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
+            ks.put(nx);
+            vs.put(nx + TB);
+        }
+        __syncthreads();
+    }
+    l += other_half(l);
+    if (r >= a.R) return;
+    const long hrow = ((long)pl.b * a.Hkv + pl.kh) * a.R + r;       // = ((b * H + head) * Sq + pos)
+    if (a.nsplit > 1) {
+        const long prow = (long)pl.split * a.B * a.Hkv * a.R + hrow;
+        float* po = a.part + prow * D;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<float4*>(po + d * 32 + 8 * q4 + 4 * h) =
+                    make_float4(acc[d][4 * q4], acc[d][4 * q4 + 1], acc[d][4 * q4 + 2], acc[d][4 * q4 + 3]);
+        if (h == 0) {
+            a.part_ml[prow * 2] = m;
+            a.part_ml[prow * 2 + 1] = l;
+        }
+        return;
+    }
+    const float inv = row_ok && l != 0.f ? 1.f / l : 0.f;
+    if (h == 0 && a.lse) a.lse[hrow] = row_ok && l != 0.f ? m - p_shift<T>() + log2f(l) : INFINITY;
+    const long orow = (((long)pl.b * a.Sq + pos) * a.H + pl.kh * a.G + g) * D * es;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const long at = (d * 32 + 8 * q4 + 4 * h) * es;
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            if (row_ok && l != 0.f)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = acc[d][4 * q4 + j] * inv;
+            if (a.ocopy) store4<T>(a.ocopy + orow + at, o[0], o[1], o[2], o[3]);
+            if (a.residual && row_ok) o += load4<T>(qrow + at);
+            store4<T>(a.o + orow + at, o[0], o[1], o[2], o[3]);
+        }
+}
+
+// joins the splits of a row: D / 4 lanes per row
+template <typename T, int D>
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
+    constexpr int LPR = D / 4;
+    const long rows = (long)a.B * a.Hkv * a.R;
+    const long row = (blockIdx.x * 256L + threadIdx.x) / LPR;
+    const int d4 = threadIdx.x % LPR;
+    if (row >= rows) return;
+    const int b = (int)(row / ((long)a.H * a.Sq));
+    const int rest = (int)(row - (long)b * a.H * a.Sq), head = rest / a.Sq, pos = rest - head * a.Sq;
+    int ql, kl;
+    lens(a, b, ql, kl);
+    float m = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+        const long at = s * rows + row;
+        const float wgt = exp2_raw(a.part_ml[at * 2] - mu);
+        l = fmaf(wgt, a.part_ml[at * 2 + 1], l);
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + at * D + d4 * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(wgt, p[j], o[j]);
+    }
+    const bool ok = pos < ql && l != 0.f;
+    if (d4 == 0 && a.lse) a.lse[row] = ok ? m - p_shift<T>() + log2f(l) : INFINITY;
+    const float inv = ok ? 1.f / l : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = ok ? o[j] * inv : 0.f;
+    const long es = sizeof(T), at = ((((long)b * a.Sq + pos) * a.H + head) * D + d4 * 4) * es;
+    if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
+    if (a.residual && pos < ql) o += load4<T>(a.q + (b * a.q_sb + pos * a.q_ss + head * a.q_sh + d4 * 4) * es);
+    store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
+}
+
+// ------------------------------------------------------------------------------------------------ backward, query side
+// The forward's shape; delta_i from the saved o, kept for the key side.
+template <typename T, int D, int NW, int KT>
+__global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int TB = KT * pitch<T, D>();
+    const Place pl = place(a, a.causal);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+    int ql, kl;
+    lens(a, pl.b, ql, kl);
+    const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
+    const int g = r / a.Sq, pos = r - g * a.Sq;
+    const bool row_ok = r < a.R && pos < ql;
+    const int off = kl - ql;
+    int lo, hi, kend = kl;
+    span(a, r0, min(r0 + NW * 32, a.R), lo, hi);
+    if (a.causal) kend = min(kl, min(hi, ql - 1) + off + 1);
+    if (lo >= ql) kend = 0;
+    int t0 = 0, t1 = (max(kend, 0) + KT - 1) / KT;
+    if (a.nsplit > 1) {
+        t0 = pl.split * a.split_tiles;
+        t1 = min(t1, t0 + a.split_tiles);
+    }
+    const long es = sizeof(T);
+    const int head = pl.kh * a.G + g;
+    const char* kb = a.k + (pl.b * a.k_sb + pl.kh * a.k_sh) * es;
+    const char* vb = a.v + (pl.b * a.v_sb + pl.kh * a.v_sh) * es;
+    const char* grow = a.doo + (pl.b * a.g_sb + pos * a.g_ss + head * a.g_sh) * es;
+    const Frag<T, D> qf = load_frag<T, D>(a.q + (pl.b * a.q_sb + pos * a.q_ss + head * a.q_sh) * es, row_ok);
+    const Frag<T, D> gf = load_frag<T, D>(grow, row_ok);
+    const long hrow = ((long)pl.b * a.Hkv + pl.kh) * a.R + r;
+    const long orow = (((long)pl.b * a.Sq + pos) * a.H + head) * D * es;
+    float dl, lse = INFINITY;
+    {
+        const Frag<T, D> of = load_frag<T, D>(a.att + orow, row_ok);
+        dl = dot_frag<T, D>(gf, of);
+        if (row_ok) lse = a.lse[hrow];
+        if (h == 0 && r < a.R && pl.split == 0) a.delta[hrow] = dl;
+    }
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) acc[d] = zero16();
+    const int klast = a.causal ? min(kl, pos + off + 1) : kl;
+
+    Stage<T, D, KT, NW * 64> ks, vs;
+    if (t0 < t1) {
+        ks.load(kb, a.k_ss * es, t0 * KT, kl);
+        vs.load(vb, a.v_ss * es, t0 * KT, kl);
+        ks.put(smem);
+        vs.put(smem + TB);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const char* kt = smem + ((t - t0) & 1) * 2 * TB;
+        const char* vt = kt + TB;
+        if (t + 1 < t1) {
+            ks.load(kb, a.k_ss * es, (t + 1) * KT, kl);
+            vs.load(vb, a.v_ss * es, (t + 1) * KT, kl);
+        }
+        const int k0 = t * KT;
+        const bool edge = k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1);
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+            f32x16 s = mul_rows<T, D>(kt, u * 32, qf, zero16());
+            f32x16 dp = mul_rows<T, D>(vt, u * 32, gf, zero16());
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = exp2_raw(fmaf(s[i], a.c, -lse)) * (dp[i] - dl);
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + u * 32 + acc_row(i, h) >= klast) s[i] = 0.f;
+            }
+            mul_cols<T, D>(kt, u * 32, s, acc);
+        }
+        if (t + 1 < t1) {
+            char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
+            ks.put(nx);
+            vs.put(nx + TB);
+        }
+        __syncthreads();
+    }
+    if (r >= a.R) return;
+    float* po = a.nsplit > 1 ? a.part + ((long)pl.split * a.B * a.Hkv * a.R + hrow) * D : nullptr;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int ch = d * 32 + 8 * q4 + 4 * h;
+            f32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = row_ok ? acc[d][4 * q4 + j] * a.scale : 0.f;
+            if (po) {
+                *reinterpret_cast<f32x4*>(po + ch) = o;
+            } else {
+                if (a.residual && row_ok) o += load4<T>(grow + ch * es);
+                store4<T>(a.dq + orow + ch * es, o[0], o[1], o[2], o[3]);
+            }
+        }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
+    constexpr int LPR = D / 4;
+    const long rows = (long)a.B * a.Hkv * a.R;
+    const long row = (blockIdx.x * 256L + threadIdx.x) / LPR;
+    const int d4 = threadIdx.x % LPR;
+    if (row >= rows) return;
+    const int b = (int)(row / ((long)a.H * a.Sq));
+    const int rest = (int)(row - (long)b * a.H * a.Sq), head = rest / a.Sq, pos = rest - head * a.Sq;
+    int ql, kl;
+    lens(a, b, ql, kl);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * D + d4 * 4);
+    const long es = sizeof(T);
+    if (a.residual && pos < ql) o += load4<T>(a.doo + (b * a.g_sb + pos * a.g_ss + head * a.g_sh + d4 * 4) * es);
+    store4<T>(a.dq + ((((long)b * a.Sq + pos) * a.H + head) * D + d4 * 4) * es, o[0], o[1], o[2], o[3]);
+}
+
+// ------------------------------------------------------------------------------------------------ backward, key side
+// NW waves of 32 keys; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
+template <typename T, int D, int NW, int RT>
+__global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int TB = RT * pitch<T, D>(), BUF = 2 * TB + RT * 8;
+    const Place pl = place(a, false);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+    int ql, kl;
+    lens(a, pl.b, ql, kl);
+    const int off = kl - ql;
+    const int key0 = pl.tile * NW * 32, key = key0 + w * 32 + (lane & 31);
+    const bool key_ok = key < kl;
+    const long es = sizeof(T);
+    const Frag<T, D> kf = load_frag<T, D>(a.k + (pl.b * a.k_sb + key * a.k_ss + pl.kh * a.k_sh) * es, key_ok);
+    const Frag<T, D> vf = load_frag<T, D>(a.v + (pl.b * a.v_sb + key * a.v_ss + pl.kh * a.v_sh) * es, key_ok);
+    const char* qb = a.q + (pl.b * a.q_sb + (long)pl.kh * a.G * a.q_sh) * es;
+    const char* gb = a.doo + (pl.b * a.g_sb + (long)pl.kh * a.G * a.g_sh) * es;
+    const long hrow0 = ((long)pl.b * a.Hkv + pl.kh) * a.R;
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = zero16();
+
+    int t1 = (a.R + RT - 1) / RT, t = 0;
+    if (a.nsplit > 1) {
+        t = pl.split * a.split_tiles;
+        t1 = min(t1, t + a.split_tiles);
+    }
+    if (key0 >= kl) t = t1;
+    // the next tile of rows with a valid pair, from t on
+    auto next = [&](int t) {
+        for (; t < t1; ++t) {
+            int lo, hi;
+            span(a, t * RT, min(t * RT + RT, a.R), lo, hi);
+            if (lo < ql && (!a.causal || min(hi, ql - 1) + off >= key0)) break;
+        }
+        return t;
+    };
+    constexpr float unshift = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.f;
+    Stage<T, D, RT, NW * 64> qs, gs;
+    float st_lse = 0.f, st_dl = 0.f;
+    auto request = [&](int t) {
+        qs.load_rows(qb, a.q_ss * es, a.q_sh * es, t * RT, a.R, a.Sq, ql);
+        gs.load_rows(gb, a.g_ss * es, a.g_sh * es, t * RT, a.R, a.Sq, ql);
+        if (threadIdx.x < RT) {
+            const int r = t * RT + threadIdx.x;
+            const bool ok = r < a.R && r - r / a.Sq * a.Sq < ql;
+            st_lse = ok ? a.lse[hrow0 + r] - p_shift<T>() : INFINITY;
+            st_dl = ok ? a.delta[hrow0 + r] * unshift : 0.f;
+        }
+    };
+    auto put = [&](char* buf) {
+        qs.put(buf);
+        gs.put(buf + TB);
+        if (threadIdx.x < RT) {
+            reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
+            reinterpret_cast<float*>(buf + 2 * TB)[RT + threadIdx.x] = st_dl;
+        }
+    };
+    t = next(t);
+    if (t < t1) {
+        request(t);
+        put(smem);
+    }
+    __syncthreads();
+    int cur = 0;
+    while (t < t1) {
+        const char* buf = smem + cur * BUF;
+        const int tn = next(t + 1);
+        if (tn < t1) request(tn);
+        int lo, hi;
+        span(a, t * RT, min(t * RT + RT, a.R), lo, hi);
+        const bool edge = a.causal && lo + off < key0 + NW * 32 - 1;
+#pragma unroll
+        for (int u = 0; u < RT / 32; ++u) {
+            f32x16 s = mul_rows<T, D>(buf, u * 32, kf, zero16());
+            f32x16 dp = mul_rows<T, D>(buf + TB, u * 32, vf, zero16());
+            const float* st = reinterpret_cast<const float*>(buf + 2 * TB) + u * 32 + 4 * h;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 8 * q4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * q4 + j] = exp2_raw(fmaf(s[4 * q4 + j], a.c, -ls[j]));
+            }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = t * RT + u * 32 + acc_row(i, h), p = r - r / a.Sq * a.Sq;
+                    if (p + off < key) s[i] = 0.f;
+                }
+            }
+            mul_cols<T, D>(buf + TB, u * 32, s, dv);
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                const f32x4 dl = *reinterpret_cast<const f32x4*>(st + RT + 8 * q4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * q4 + j] *= fmaf(dp[4 * q4 + j], unshift, -dl[j]);
+            }
+            mul_cols<T, D>(buf, u * 32, s, dk);
+        }
+        if (tn < t1) put(smem + (cur ^ 1) * BUF);
+        __syncthreads();
+        cur ^= 1;
+        t = tn;
+    }
+    if (key >= a.Sk) return;
+    const long krow = ((long)pl.b * a.Sk + key) * a.Hkv + pl.kh;
+    const long part0 = (long)pl.split * a.B * a.Sk * a.Hkv + krow, total = (long)a.nsplit * a.B * a.Sk * a.Hkv;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const int ch = d * 32 + 8 * q4 + 4 * h;
+            f32x4 x, y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = key_ok ? dk[d][4 * q4 + j] * a.scale : 0.f;
+                y[j] = key_ok ? dv[d][4 * q4 + j] * unshift : 0.f;
+            }
+            if (a.nsplit > 1) {
+                *reinterpret_cast<f32x4*>(a.part + part0 * D + ch) = x;
+                *reinterpret_cast<f32x4*>(a.part + (total + part0) * D + ch) = y;
+            } else {
+                store4<T>(a.dk + (krow * D + ch) * es, x[0], x[1], x[2], x[3]);
+                store4<T>(a.dv + (krow * D + ch) * es, y[0], y[1], y[2], y[3]);
+            }
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dkv_join_kernel(Args a, long n4) {
+    const long e = blockIdx.x * 256L + threadIdx.x;
+    if (e >= n4) return;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    const f32x4* p = reinterpret_cast<const f32x4*>(a.part);
+    for (int s = 0; s < a.nsplit; ++s) {
+        x += p[s * n4 + e];
+        y += p[(a.nsplit + s) * n4 + e];
+    }
+    store4<T>(a.dk + e * 4 * sizeof(T), x[0], x[1], x[2], x[3]);
+    store4<T>(a.dv + e * 4 * sizeof(T), y[0], y[1], y[2], y[3]);
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+struct Plan {
+    int nw, tile, ntiles, nsplit, split_tiles;      // waves per workgroup, contraction rows per tile, tiles of own rows
+    size_t lds;
+};
+
+// `rows` own rows in tiles of 32 per wave, `len` rows to walk.  Four waves share what they walk; where that leaves most
+// of the card idle, one wave per workgroup and the walk cut into pieces that a second launch joins.
+static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats) {
+    Plan p;
+    const long wg4 = nbh * ((rows + 127) / 128);
+    p.nw = wg4 >= 256 ? 4 : 1;
+    p.tile = p.nw == 4 && esize * D <= 256 ? 64 : 32;
+    p.ntiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
+    p.nsplit = 1;
+    const int tiles = (len + p.tile - 1) / p.tile;
+    const long wg = nbh * p.ntiles, want = p.nw == 4 ? 256 : 1024;
+    if (wg > 0 && wg < want && tiles > 1) {
+        long ns = (want + wg - 1) / wg;
+        if (ns > tiles / 2) ns = tiles / 2;           // at least two tiles per piece
+        if (ns > 64) ns = 64;
+        if (ns > 1) p.nsplit = (int)ns;
+    }
+    p.split_tiles = (tiles + p.nsplit - 1) / p.nsplit;
+    if (p.split_tiles < 1) p.split_tiles = 1;
+    p.nsplit = tiles > 0 ? (tiles + p.split_tiles - 1) / p.split_tiles : 1;
+    p.lds = 2 * ((size_t)2 * p.tile * (D * esize + 16) + (stats ? p.tile * 8 : 0));
+    return p;
+}
+
+static size_t esize_of(int dtype) { return dtype == CMVAE_F32 ? 4 : 2; }
+
+struct Sizes {
+    Plan f, q, k;
+    size_t fwd, bwd;
+};
+static Sizes sizes_of(const cmvae_set_attn& d) {
+    Sizes z;
+    const int es = (int)esize_of(d.dtype), G = d.H / d.Hkv;
+    const long nbh = (long)d.B * d.Hkv;
+    const int R = G * d.Sq;
+    z.f = make_plan(es, d.D, nbh, R, d.Sk, false);
+    z.q = z.f;
+    z.k = make_plan(es, d.D, nbh, d.Sk, R, true);
+    const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
+    z.fwd = z.f.nsplit > 1 ? z.f.nsplit * rows * (d.D + 2) * 4 : 0;
+    const size_t bq = z.q.nsplit > 1 ? z.q.nsplit * rows * d.D * 4 : 0;
+    const size_t bk = z.k.nsplit > 1 ? (size_t)z.k.nsplit * 2 * keys * d.D * 4 : 0;
+    z.bwd = bq > bk ? bq : bk;                    // the key side's launches follow the query side's on the same stream
+    return z;
+}
+
+template <typename K>
+static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a, void* stream, const char* what) {
+    if (blocks == 0) return 0;                    // no keys: there is no key side
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return set_error("%s: %s", what, hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, a);
+    return check_launch(what);
+}
+
+static void use(Args& a, const Plan& p) {
+    a.ntiles = p.ntiles;
+    a.nsplit = p.nsplit;
+    a.split_tiles = p.split_tiles;
+}
+
+template <typename T, int D>
+static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
+    constexpr int T4 = sizeof(T) * D <= 256 ? 64 : 32;
+    const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R;
+    use(a, z.f);
+    a.part = ws;
+    a.part_ml = ws + (size_t)a.nsplit * rows * D;
+    const long blocks = nbh * a.ntiles * a.nsplit;
+    int e = z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
+                        : launch(fwd_kernel<T, D, 1, 32>, blocks, 64, z.f.lds, a, stream, "set_attention fwd_kernel");
+    if (e || a.nsplit == 1) return e;
+    return launch(fwd_join_kernel<T, D>, (rows * (D / 4) + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
+}
+
+template <typename T, int D>
+static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
+    constexpr int T4 = sizeof(T) * D <= 256 ? 64 : 32;
+    const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R, keys = nbh * a.Sk;
+    a.part = ws;
+    use(a, z.q);
+    long blocks = nbh * a.ntiles * a.nsplit;
+    int e = z.q.nw == 4 ? launch(dq_kernel<T, D, 4, T4>, blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
+                        : launch(dq_kernel<T, D, 1, 32>, blocks, 64, z.q.lds, a, stream, "set_attention dq_kernel");
+    if (e) return e;
+    if (a.nsplit > 1 &&
+        (e = launch(dq_join_kernel<T, D>, (rows * (D / 4) + 255) / 256, 256, 0, a, stream, "set_attention dq_join_kernel")))
+        return e;
+    use(a, z.k);
+    blocks = nbh * a.ntiles * a.nsplit;
+    e = z.k.nw == 4 ? launch(dkv_kernel<T, D, 4, T4>, blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
+                    : launch(dkv_kernel<T, D, 1, 32>, blocks, 64, z.k.lds, a, stream, "set_attention dkv_kernel");
+    if (e || a.nsplit == 1) return e;
+    const long n4 = keys * D / 4;
+    hipLaunchKernelGGL(dkv_join_kernel<T>, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a, n4);
+    return check_launch("set_attention dkv_join_kernel");
+}
+
+static bool aligned(const void* p, const int64_t* s, int dtype, int extra) {
+    const int m = 16 / (int)esize_of(dtype);
+    for (int i = 0; i < 3; ++i)
+        if (s[i] % m || s[i] < 0) return false;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && extra % m == 0;
+}
+
+static int check_desc(const char* who, const cmvae_set_attn* d) {
+    CMVAE_REQUIRE(d != nullptr, "%s: NULL descriptor", who);
+    CMVAE_REQUIRE(d->dtype == CMVAE_F32 || d->dtype == CMVAE_BF16 || d->dtype == CMVAE_F16, "%s: dtype %d", who, d->dtype);
+    CMVAE_REQUIRE(d->D == 64 || d->D == 128, "%s: heads of %d channels (64 or 128 are supported)", who, d->D);
+    CMVAE_REQUIRE(d->B >= 1 && d->Sq >= 1 && d->Sk >= 0 && d->H >= 1 && d->Hkv >= 1 && d->H % d->Hkv == 0,
+                  "%s: B=%d Sq=%d Sk=%d heads=%d key heads=%d", who, d->B, d->Sq, d->Sk, d->H, d->Hkv);
+    CMVAE_REQUIRE((long)d->H / d->Hkv * d->Sq < (1L << 30) && d->Sk < (1 << 30), "%s: more than 2^30 rows per key head", who);
+    CMVAE_REQUIRE(d->scale >= 1e-30f && d->scale <= 1e30f, "%s: scale %g (a positive finite number)", who, (double)d->scale);
+    const Sizes z = sizes_of(*d);
+    const long nbh = (long)d->B * d->Hkv;
+    CMVAE_REQUIRE(nbh * z.f.ntiles * z.f.nsplit < (1L << 31) && nbh * z.k.ntiles * z.k.nsplit < (1L << 31) &&
+                      nbh * (d->H / d->Hkv) * d->Sq * (d->D / 4) / 256 < (1L << 31) - 1 &&
+                      nbh * d->Sk * (d->D / 4) / 256 < (1L << 31) - 1,
+                  "%s: the problem needs more than 2^31 workgroups", who);
+    return 0;
+}
+
+static Args args_of(const cmvae_set_attn& d) {
+    Args a = {};
+    a.q = (const char*)d.q; a.k = (const char*)d.k; a.v = (const char*)d.v;
+    a.doo = (const char*)d.dO;
+    a.o = (char*)d.o; a.ocopy = (char*)d.attn;
+    a.att = (const char*)(d.residual ? d.attn : d.o);
+    a.dq = (char*)d.dq; a.dk = (char*)d.dk; a.dv = (char*)d.dv;
+    a.lse = d.lse; a.delta = d.delta;
+    a.q_len = d.q_len; a.k_len = d.k_len;
+    a.q_sb = d.q_stride[0]; a.q_ss = d.q_stride[1]; a.q_sh = d.q_stride[2];
+    a.k_sb = d.k_stride[0]; a.k_ss = d.k_stride[1]; a.k_sh = d.k_stride[2];
+    a.v_sb = d.v_stride[0]; a.v_ss = d.v_stride[1]; a.v_sh = d.v_stride[2];
+    a.g_sb = d.dO_stride[0]; a.g_ss = d.dO_stride[1]; a.g_sh = d.dO_stride[2];
+    a.B = d.B; a.Sq = d.Sq; a.Sk = d.Sk; a.H = d.H; a.Hkv = d.Hkv;
+    a.G = d.H / d.Hkv;
+    a.R = a.G * d.Sq;
+    a.causal = d.causal != 0;
+    a.residual = d.residual != 0;
+    a.scale = d.scale;
+    a.c = d.scale * LOG2E;
+    return a;
+}
+
+}  // namespace sa
+}  // namespace cmvae
+
+using namespace cmvae;
+
+#define SA_DISPATCH(fn)                                                                        \
+    switch (d->dtype * 1000 + d->D) {                                                          \
+        case CMVAE_F32 * 1000 + 64: return sa::fn<float, 64>(a, z, (float*)workspace, stream);  \
+        case CMVAE_F32 * 1000 + 128: return sa::fn<float, 128>(a, z, (float*)workspace, stream); \
+        case CMVAE_BF16 * 1000 + 64: return sa::fn<__bf16, 64>(a, z, (float*)workspace, stream); \
+        case CMVAE_BF16 * 1000 + 128: return sa::fn<__bf16, 128>(a, z, (float*)workspace, stream); \
+        case CMVAE_F16 * 1000 + 64: return sa::fn<_Float16, 64>(a, z, (float*)workspace, stream); \
+        default: return sa::fn<_Float16, 128>(a, z, (float*)workspace, stream);                 \
+    }
+
+extern "C" size_t cmvae_set_attention_workspace_bytes(const cmvae_set_attn* d, int backward) {
+    cmvae::clear_stale_error();
+    if (sa::check_desc("cmvae_set_attention_workspace_bytes", d)) return 0;
+    const sa::Sizes z = sa::sizes_of(*d);
+    return backward ? z.bwd : z.fwd;
+}
+
+extern "C" int cmvae_set_attention_fwd(const cmvae_set_attn* d, void* workspace, size_t workspace_bytes, void* stream) {
+    cmvae::clear_stale_error();
+    if (int e = sa::check_desc("cmvae_set_attention_fwd", d)) return e;
+    CMVAE_REQUIRE(d->q && d->o && (d->Sk == 0 || (d->k && d->v)), "cmvae_set_attention_fwd: NULL tensor");
+    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype, 0) && sa::aligned(d->k, d->k_stride, d->dtype, 0) &&
+                      sa::aligned(d->v, d->v_stride, d->dtype, 0) && ((uintptr_t)d->o & 15) == 0 && ((uintptr_t)d->attn & 15) == 0,
+                  "cmvae_set_attention_fwd: rows must start at multiples of 16 bytes");
+    const sa::Sizes z = sa::sizes_of(*d);
+    CMVAE_REQUIRE(z.fwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.fwd),
+                  "cmvae_set_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, z.fwd);
+    sa::Args a = sa::args_of(*d);
+    SA_DISPATCH(run_fwd)
+}
+
+extern "C" int cmvae_set_attention_bwd(const cmvae_set_attn* d, void* workspace, size_t workspace_bytes, void* stream) {
+    cmvae::clear_stale_error();
+    if (int e = sa::check_desc("cmvae_set_attention_bwd", d)) return e;
+    CMVAE_REQUIRE(d->q && d->dO && d->lse && d->delta && d->dq && (d->residual ? (const void*)d->attn : d->o) &&
+                      (d->Sk == 0 || (d->k && d->v && d->dk && d->dv)),
+                  "cmvae_set_attention_bwd: NULL tensor");
+    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype, 0) && sa::aligned(d->k, d->k_stride, d->dtype, 0) &&
+                      sa::aligned(d->v, d->v_stride, d->dtype, 0) && sa::aligned(d->dO, d->dO_stride, d->dtype, 0) &&
+                      (((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv | (uintptr_t)d->o | (uintptr_t)d->attn) & 15) == 0,
+                  "cmvae_set_attention_bwd: rows must start at multiples of 16 bytes");
+    const sa::Sizes z = sa::sizes_of(*d);
+    CMVAE_REQUIRE(z.bwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bwd),
+                  "cmvae_set_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, z.bwd);
+    sa::Args a = sa::args_of(*d);
+    SA_DISPATCH(run_bwd)
+}

@@ -290,6 +290,33 @@ int cmvae_attention_qkv_fwd(const float* QKV, int B, int S, int heads, float sca
 int cmvae_attention_qkv_bwd(const float* QKV, const float* lse, const float* dO, int B, int S, int heads,
                             float scale, float* dQKV, float* delta, void* stream);
 
+/* ==== set attention for any set sizes, padded sets and shared key heads, with its backward pass (the softmax core of
+ * MAB.forward, omniglot/module.py:92-99, beyond the shapes of cmvae_attention_*):
+ *   s_ij = scale q_i . k_j;  valid (i, j): i < q_len[b], j < k_len[b] and, if causal, j <= i + k_len[b] - q_len[b];
+ *   o_i = softmax over the valid j (no valid j: zeros) . v  (+ q_i if residual);  rows i >= q_len[b] of o are zeros.
+ * q, dO [B,Sq,H,D] and k, v [B,Sk,Hkv,D] with strides {batch, row, head} in elements (channels are adjacent, rows start
+ * at multiples of 16 bytes); D 64 or 128, H a multiple of Hkv (query head h reads key head h / (H / Hkv)).  o, attn, dq
+ * [B,Sq,H,D] and dk, dv [B,Sk,Hkv,D] are dense.  q_len, k_len: int32 [B] or NULL (all rows), clamped to the tensors.
+ * Values of rows behind a length are not read.  lse, delta: fp32 [B,H,Sq].  Forward: lse may be NULL; attn, if not NULL,
+ * receives o without the residual.  Backward: reads o (residual: attn) and lse of the forward, writes delta (scratch),
+ * dq, dk, dv; gradients of rows behind a length are zeros.                                                          */
+#define CMVAE_F32 0
+#define CMVAE_BF16 1
+#define CMVAE_F16 2
+typedef struct cmvae_set_attn {
+    int32_t dtype, B, Sq, Sk, H, Hkv, D, causal, residual;
+    float scale;                                       /* > 0 */
+    const void *q, *k, *v, *dO;
+    int64_t q_stride[3], k_stride[3], v_stride[3], dO_stride[3];
+    const int32_t *q_len, *k_len;
+    void *o, *attn;
+    float *lse, *delta;
+    void *dq, *dk, *dv;
+} cmvae_set_attn;
+size_t cmvae_set_attention_workspace_bytes(const cmvae_set_attn* desc, int backward);   /* 0 on a bad descriptor, too */
+int cmvae_set_attention_fwd(const cmvae_set_attn* desc, void* workspace, size_t workspace_bytes, void* stream);
+int cmvae_set_attention_bwd(const cmvae_set_attn* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ==== NOTEARS-MLP causal layer on bulk rows (CausalEncoder.forward on [B*N,64], omniglot/module.py:165-188,
  * LocallyConnected :232-288).  hid [rows,2048] = elu(fc1(x)) comes from cmvae_linear_fwd(act=2);
  * eps[r][j] = x[r][j] - (sum_m hid[r][32j+m] w2[j][m] + b2[j]).
