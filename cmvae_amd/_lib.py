@@ -167,6 +167,10 @@ SIGNATURES = {
                                     c_float, c_float, c_float, c_void_p]),
     'cmvae_adam_step': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_float,
                                 c_float, c_float, c_void_p]),
+    'cmvae_adamw_step': (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                 ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                 c_void_p]),
+    'cmvae_adamw_state_values': (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     'cmvae_em_seed_draw_host': (c_int, [c_void_p, ctypes.POINTER(c_int), c_int, c_int, c_int, c_void_p, c_void_p]),
 }
 

@@ -340,6 +340,26 @@ int cmvae_adam_step_dev(float* param, const float* grad, float* exp_avg, float* 
                         const int64_t* step_dev, float lr, float beta1, float beta2, float eps, float weight_decay,
                         void* stream);
 
+/* ==== AdamW (decoupled weight decay) over many tensors, with states in 32 or in 8 bits:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
+ * tensors_host: `count` descriptors in HOST memory, read before the call returns (the kernels get them as launch arguments);
+ * param and grad are dense, of one dtype (CMVAE_F32 / BF16 / F16), no two tensors overlap.  exp_avg, exp_avg_sq: flat, the
+ * states of a tensor start at `state` (a multiple of 256) and take its n values rounded up to a multiple of 256.
+ * state_bits 32: fp32.  8: one byte per value, scales [2][state_len / 256] fp32 (first moment's, then second's); exp_avg is
+ * e4m3 of m / scale, exp_avg_sq = c stands for scale * 2^((c >> 3) - 31) * (1 + (c & 7) / 8), 0 for 0, 255 for a value that
+ * is not finite (read as infinity).  step counts from 1; step_dev, if not NULL, is read in its place on the device (HIP graphs).          */
+typedef struct cmvae_adamw_tensor {
+    void* param;
+    const void* grad;
+    int64_t n, state, dtype;
+} cmvae_adamw_tensor;
+int cmvae_adamw_step(const cmvae_adamw_tensor* tensors_host, int count, int state_bits, void* exp_avg, void* exp_avg_sq,
+                     float* scales, int64_t state_len, int64_t step, const int64_t* step_dev, double lr, double beta1,
+                     double beta2, double eps, double weight_decay, void* stream);
+/* the fp32 values that 8-bit states stand for */
+int cmvae_adamw_state_values(const void* exp_avg, const void* exp_avg_sq, const float* scales, int64_t state_len,
+                             float* exp_avg_out, float* exp_avg_sq_out, void* stream);
+
 /* ==== BatchNorm (training statistics over the whole meta-batch) on channels-last [rows,64]
  * nn.BatchNorm2d after every conv (omniglot/module.py:15,20,25,30,51,55,59).  The conv GEMM
  * emits per-block partial sums; these finish the job.                                        */
