@@ -45,7 +45,16 @@ class SetAttnDesc(ctypes.Structure):
                [(n, c_void_p) for n in ('q_len', 'k_len', 'o', 'attn', 'lse', 'delta', 'dq', 'dk', 'dv')]
 
 
+class GroupNormDesc(ctypes.Structure):
+    """struct cmvae_group_norm (include/cmvae_abi.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'wdtype', 'act', 'N', 'P', 'C', 'G')] + [('eps', c_float)] + \
+               [(n, c_void_p) for n in ('x', 'weight', 'bias', 'dy')] + \
+               [(n, c_int64 * 2) for n in ('x_stride', 'dy_stride')] + \
+               [(n, c_void_p) for n in ('y', 'stats', 'dx', 'dweight', 'dbias')]
+
+
 _PS = ctypes.POINTER(SetAttnDesc)
+_PN = ctypes.POINTER(GroupNormDesc)
 
 # name -> (restype, argtypes); must list every symbol of include/cmvae_abi.h
 SIGNATURES = {
@@ -171,6 +180,9 @@ SIGNATURES = {
                                  ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                  c_void_p]),
     'cmvae_adamw_state_values': (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    'cmvae_group_norm_workspace_bytes': (c_size_t, [_PN, c_int]),
+    'cmvae_group_norm_fwd': (c_int, [_PN, c_void_p, c_size_t, c_void_p]),
+    'cmvae_group_norm_bwd': (c_int, [_PN, c_void_p, c_size_t, c_void_p]),
     'cmvae_em_seed_draw_host': (c_int, [c_void_p, ctypes.POINTER(c_int), c_int, c_int, c_int, c_void_p, c_void_p]),
 }
 

@@ -1,0 +1,706 @@
+// Group norm with an activation on channels-last rows, and its backward pass: cmvae_group_norm_{fwd,bwd}.
+//
+//   per sample n and group g of C / G channels: mean and biased variance over the sample's P pixels x C / G channels,
+//   xhat = (x - mean) rstd,  z = xhat w_c + b_c,  y = act(z)
+//   dz = dy act'(z),  db_c = sum dz,  dw_c = sum dz xhat,
+//   dx = rstd (dz w_c - m1 - xhat m2),   m1, m2 = means over the group of dz w_c and dz w_c xhat
+//
+// Both directions are bound by memory.  A sample whose rows fit in the registers of one workgroup is read once and written
+// once (resident kernels); a larger one takes a pass for its sums, a small launch that finishes them, and a pass that
+// applies them.  Sums are kept per channel, so a group may end anywhere in a thread's vector of channels.
+//
+// The forward's sums of x and x^2 are fp64 (full rate on this card, and two instructions of the few per value): no
+// shift, no second pass, and a variance that survives a mean thousands of deviations away.  The mean is kept as two fp32
+// numbers for the same reason.  The backward's sums are of mixed sign and fp32 in a thread, fp64 where threads meet.
+// Sums are added in a fixed order: every run gives the same bits.
+#include "common.h"
+
+#include <cmath>
+#include <type_traits>
+
+namespace cmvae {
+namespace gn {
+
+struct Args {
+    const void *x, *dy, *w, *b;
+    void *y, *dx, *dw, *db;
+    float4* stats;                              // [N, G]: mean (two parts), rstd
+    double2* part;                              // forward sums [N, pc, C]
+    float2* bpart;                              // backward sums [N, pc, C]
+    float2* means;                              // m1, m2 [N, G]
+    long x_sn, x_sp, g_sn, g_sp;                // strides in elements
+    int N, P, C, G, Cg, CV, act, wtype;
+    int pc, rows_per, cc;                       // pixel pieces per sample, pixels per piece, channel pieces
+    float eps;
+};
+
+template <typename T, int V>
+struct Vec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct Vec<T, 1> {
+    typedef T type;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const typename Vec<T, V>::type& p, float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = (float)p;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = (float)p[j];
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ typename Vec<T, V>::type pack(const float (&x)[V]) {
+    typename Vec<T, V>::type p;
+    if constexpr (V == 1) {
+        p = (T)x[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[j] = (T)x[j];
+    }
+    return p;
+}
+
+__device__ __forceinline__ float param(const void* p, int type, int c, float none) {
+    if (!p) return none;
+    if (type == CMVAE_F32) return ((const float*)p)[c];
+    if (type == CMVAE_BF16) return (float)((const __bf16*)p)[c];
+    return (float)((const _Float16*)p)[c];
+}
+__device__ __forceinline__ void put_param(void* p, int type, int c, double v) {
+    if (!p) return;
+    if (type == CMVAE_F32) ((float*)p)[c] = (float)v;
+    else if (type == CMVAE_BF16) ((__bf16*)p)[c] = (__bf16)(float)v;
+    else ((_Float16*)p)[c] = (_Float16)(float)v;
+}
+
+__device__ __forceinline__ float act_fwd(float z, int act) {
+    switch (act) {
+        case 1: return z > 0.f ? z : (z != z ? z : 0.f);
+        case 2: return elu1(z);
+        case 3: return z / (1.f + __expf(-z));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case 1: return z > 0.f ? 1.f : 0.f;
+        case 2: return z > 0.f ? 1.f : __expf(z);
+        case 3: {
+            const float s = 1.f / (1.f + __expf(-z));
+            return s * fmaf(z, 1.f - s, 1.f);
+        }
+        default: return 1.f;
+    }
+}
+
+__device__ __forceinline__ float4 make_stats(double s1, double s2, double m, float eps) {
+    const double mean = s1 / m, var = fmax(s2 / m - mean * mean, 0.0);
+    const float hi = (float)mean;
+    return make_float4(hi, (float)(mean - (double)hi), (float)(1.0 / sqrt(var + (double)eps)), 0.f);
+}
+
+// a thread's V channels: what normalises them
+template <int V>
+struct Channel {
+    float mh[V], ml[V], rs[V], w[V], b[V];
+};
+template <int V>
+__device__ __forceinline__ void load_channels(const Args& a, const float4* st, int c0, Channel<V>& k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float4 s = st[(c0 + j) / a.Cg];
+        k.mh[j] = s.x; k.ml[j] = s.y; k.rs[j] = s.z;
+        k.w[j] = param(a.w, a.wtype, c0 + j, 1.f);
+        k.b[j] = param(a.b, a.wtype, c0 + j, 0.f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ resident
+// One workgroup per sample; thread t holds vectors t, t + A, t + 2A ... of the sample's P * CV, A = the largest multiple
+// of CV up to the workgroup: its channels are the same in all of them.
+template <typename T, int V, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
+    extern __shared__ __align__(16) char smem[];
+    double2* red = reinterpret_cast<double2*>(smem);                       // [rows][C], then [C]
+    float4* st = reinterpret_cast<float4*>(smem + (size_t)THREADS * V * sizeof(double2));
+    typedef typename Vec<T, V>::type TV;
+    const int n = blockIdx.x, t = threadIdx.x;
+    const int rows = THREADS / a.CV, A = rows * a.CV;
+    const int row = t / a.CV, c0 = (t - row * a.CV) * V;
+    const bool on = t < A;
+    const T* x = (const T*)a.x + n * a.x_sn + c0;
+    TV hold[R];
+    double s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int p = row + i * rows;
+        if (on && p < a.P) hold[i] = *reinterpret_cast<const TV*>(x + p * a.x_sp);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (on && row + i * rows < a.P) {
+            float v[V];
+            unpack<T, V>(hold[i], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double d = (double)v[j];
+                s1[j] += d;
+                s2[j] = fma(d, d, s2[j]);
+            }
+        }
+    }
+    if (on)
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[row * a.C + c0 + j] = make_double2(s1[j], s2[j]);
+    __syncthreads();
+    for (int c = t; c < a.C; c += THREADS) {
+        double2 s = red[c];
+        for (int r = 1; r < rows; ++r) {
+            const double2 q = red[r * a.C + c];
+            s.x += q.x;
+            s.y += q.y;
+        }
+        red[c] = s;
+    }
+    __syncthreads();
+    for (int g = t; g < a.G; g += THREADS) {
+        double u = 0.0, v = 0.0;
+        for (int c = g * a.Cg; c < (g + 1) * a.Cg; ++c) {
+            u += red[c].x;
+            v += red[c].y;
+        }
+        const float4 s = make_stats(u, v, (double)a.P * a.Cg, a.eps);
+        st[g] = s;
+        if (a.stats) a.stats[(long)n * a.G + g] = s;
+    }
+    __syncthreads();
+    if (!on) return;
+    Channel<V> k;
+    load_channels<V>(a, st, c0, k);
+    T* y = (T*)a.y + (long)n * a.P * a.C + c0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int p = row + i * rows;
+        if (p < a.P) {
+            float v[V];
+            unpack<T, V>(hold[i], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                v[j] = act_fwd(fmaf((v[j] - k.mh[j] - k.ml[j]) * k.rs[j], k.w[j], k.b[j]), a.act);
+            *reinterpret_cast<TV*>(y + (long)p * a.C) = pack<T, V>(v);
+        }
+    }
+}
+
+template <typename T, int V, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void bwd_resident_kernel(Args a) {
+    extern __shared__ __align__(16) char smem[];
+    float2* red = reinterpret_cast<float2*>(smem);
+    float4* st = reinterpret_cast<float4*>(smem + (size_t)THREADS * V * sizeof(float2));
+    float2* mm = reinterpret_cast<float2*>(st + a.G);
+    typedef typename Vec<T, V>::type TV;
+    const int n = blockIdx.x, t = threadIdx.x;
+    const int rows = THREADS / a.CV, A = rows * a.CV;
+    const int row = t / a.CV, c0 = (t - row * a.CV) * V;
+    const bool on = t < A;
+    const T* x = (const T*)a.x + n * a.x_sn + c0;
+    const T* dy = (const T*)a.dy + n * a.g_sn + c0;
+    TV hx[R], hg[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int p = row + i * rows;
+        if (on && p < a.P) {
+            hx[i] = *reinterpret_cast<const TV*>(x + p * a.x_sp);
+            hg[i] = *reinterpret_cast<const TV*>(dy + p * a.g_sp);
+        }
+    }
+    for (int g = t; g < a.G; g += THREADS) st[g] = a.stats[(long)n * a.G + g];
+    __syncthreads();
+    Channel<V> k;
+    if (on) load_channels<V>(a, st, c0, k);
+    float s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (on && row + i * rows < a.P) {
+            float v[V], d[V];
+            unpack<T, V>(hx[i], v);
+            unpack<T, V>(hg[i], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
+                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
+                s1[j] += dz;
+                s2[j] = fmaf(dz, xh, s2[j]);
+            }
+        }
+    }
+    if (on)
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[row * a.C + c0 + j] = make_float2(s1[j], s2[j]);
+    __syncthreads();
+    for (int c = t; c < a.C; c += THREADS) {
+        double u = 0.0, v = 0.0;
+        for (int r = 0; r < rows; ++r) {
+            const float2 q = red[r * a.C + c];
+            u += (double)q.x;
+            v += (double)q.y;
+        }
+        const float2 s = make_float2((float)u, (float)v);
+        red[c] = s;
+        if (a.bpart) a.bpart[(long)n * a.C + c] = s;
+    }
+    __syncthreads();
+    for (int g = t; g < a.G; g += THREADS) {
+        double u = 0.0, v = 0.0;
+        for (int c = g * a.Cg; c < (g + 1) * a.Cg; ++c) {
+            const double w = (double)param(a.w, a.wtype, c, 1.f);
+            u += w * (double)red[c].x;
+            v += w * (double)red[c].y;
+        }
+        const double m = (double)a.P * a.Cg;
+        mm[g] = make_float2((float)(u / m), (float)(v / m));
+    }
+    __syncthreads();
+    if (!on) return;
+    float m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 q = mm[(c0 + j) / a.Cg];
+        m1[j] = q.x;
+        m2[j] = q.y;
+    }
+    T* dx = (T*)a.dx + (long)n * a.P * a.C + c0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int p = row + i * rows;
+        if (p < a.P) {
+            float v[V], d[V];
+            unpack<T, V>(hx[i], v);
+            unpack<T, V>(hg[i], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
+                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
+                v[j] = k.rs[j] * (fmaf(dz, k.w[j], -m1[j]) - xh * m2[j]);
+            }
+            *reinterpret_cast<TV*>(dx + (long)p * a.C) = pack<T, V>(v);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ in pieces
+struct Piece {
+    int n, pc, c0, row, rows, cw, p0, p1;
+    bool on;
+};
+template <int V>
+__device__ __forceinline__ Piece piece(const Args& a) {
+    Piece q;
+    int id = blockIdx.x;
+    const int cc = id % a.cc;
+    id /= a.cc;
+    q.pc = id % a.pc;
+    q.n = id / a.pc;
+    q.cw = min(a.CV - cc * 256, 256);                             // vectors of channels in this piece
+    q.rows = 256 / q.cw;
+    q.row = (int)threadIdx.x / q.cw;
+    q.on = q.row < q.rows;
+    q.c0 = (cc * 256 + (int)threadIdx.x - q.row * q.cw) * V;
+    q.p0 = q.pc * a.rows_per;
+    q.p1 = min(a.P, q.p0 + a.rows_per);
+    return q;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void fwd_sums_kernel(Args a) {
+    __shared__ double2 red[256 * V];
+    typedef typename Vec<T, V>::type TV;
+    const Piece q = piece<V>(a);
+    double s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
+    const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
+    if (q.on)
+#pragma unroll 4
+        for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
+            float v[V];
+            unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double d = (double)v[j];
+                s1[j] += d;
+                s2[j] = fma(d, d, s2[j]);
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[threadIdx.x * V + j] = make_double2(s1[j], s2[j]);
+    __syncthreads();
+    if (q.row != 0) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        double2 s = red[threadIdx.x * V + j];
+        for (int r = 1; r < q.rows; ++r) {
+            const double2 u = red[(threadIdx.x + r * q.cw) * V + j];
+            s.x += u.x;
+            s.y += u.y;
+        }
+        a.part[((long)q.n * a.pc + q.pc) * a.C + q.c0 + j] = s;
+    }
+}
+
+// one wave per (sample, group)
+__global__ __launch_bounds__(64) void fwd_finish_kernel(Args a) {
+    const long ng = blockIdx.x;
+    const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
+    double u = 0.0, v = 0.0;
+    const int items = a.pc * a.Cg;
+    for (int i = threadIdx.x; i < items; i += 64) {
+        const int pc = i / a.Cg, c = i - pc * a.Cg;
+        const double2 s = a.part[((long)n * a.pc + pc) * a.C + g * a.Cg + c];
+        u += s.x;
+        v += s.y;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        u += __shfl_xor(u, o);
+        v += __shfl_xor(v, o);
+    }
+    if (threadIdx.x == 0) a.stats[ng] = make_stats(u, v, (double)a.P * a.Cg, a.eps);
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void fwd_apply_kernel(Args a) {
+    typedef typename Vec<T, V>::type TV;
+    const Piece q = piece<V>(a);
+    if (!q.on) return;
+    Channel<V> k;
+    load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+    const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
+    T* y = (T*)a.y + (long)q.n * a.P * a.C + q.c0;
+#pragma unroll 4
+    for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
+        float v[V];
+        unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_fwd(fmaf((v[j] - k.mh[j] - k.ml[j]) * k.rs[j], k.w[j], k.b[j]), a.act);
+        *reinterpret_cast<TV*>(y + (long)p * a.C) = pack<T, V>(v);
+    }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
+    __shared__ float2 red[256 * V];
+    typedef typename Vec<T, V>::type TV;
+    const Piece q = piece<V>(a);
+    float s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
+    if (q.on) {
+        Channel<V> k;
+        load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+        const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
+        const T* dy = (const T*)a.dy + q.n * a.g_sn + q.c0;
+#pragma unroll 4
+        for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
+            float v[V], d[V];
+            unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
+            unpack<T, V>(*reinterpret_cast<const TV*>(dy + p * a.g_sp), d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
+                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
+                s1[j] += dz;
+                s2[j] = fmaf(dz, xh, s2[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[threadIdx.x * V + j] = make_float2(s1[j], s2[j]);
+    __syncthreads();
+    if (q.row != 0) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        double u = 0.0, v = 0.0;
+        for (int r = 0; r < q.rows; ++r) {
+            const float2 s = red[(threadIdx.x + r * q.cw) * V + j];
+            u += (double)s.x;
+            v += (double)s.y;
+        }
+        a.bpart[((long)q.n * a.pc + q.pc) * a.C + q.c0 + j] = make_float2((float)u, (float)v);
+    }
+}
+
+__global__ __launch_bounds__(64) void bwd_finish_kernel(Args a) {
+    const long ng = blockIdx.x;
+    const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
+    double u = 0.0, v = 0.0;
+    const int items = a.pc * a.Cg;
+    for (int i = threadIdx.x; i < items; i += 64) {
+        const int pc = i / a.Cg, c = g * a.Cg + i - pc * a.Cg;
+        const float2 s = a.bpart[((long)n * a.pc + pc) * a.C + c];
+        const double w = (double)param(a.w, a.wtype, c, 1.f);
+        u += w * (double)s.x;
+        v += w * (double)s.y;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        u += __shfl_xor(u, o);
+        v += __shfl_xor(v, o);
+    }
+    const double m = (double)a.P * a.Cg;
+    if (threadIdx.x == 0) a.means[ng] = make_float2((float)(u / m), (float)(v / m));
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void bwd_apply_kernel(Args a) {
+    typedef typename Vec<T, V>::type TV;
+    const Piece q = piece<V>(a);
+    if (!q.on) return;
+    Channel<V> k;
+    load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+    float m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = a.means[(long)q.n * a.G + (q.c0 + j) / a.Cg];
+        m1[j] = s.x;
+        m2[j] = s.y;
+    }
+    const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
+    const T* dy = (const T*)a.dy + q.n * a.g_sn + q.c0;
+    T* dx = (T*)a.dx + (long)q.n * a.P * a.C + q.c0;
+#pragma unroll 4
+    for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
+        float v[V], d[V];
+        unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
+        unpack<T, V>(*reinterpret_cast<const TV*>(dy + p * a.g_sp), d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
+            const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
+            v[j] = k.rs[j] * (fmaf(dz, k.w[j], -m1[j]) - xh * m2[j]);
+        }
+        *reinterpret_cast<TV*>(dx + (long)p * a.C) = pack<T, V>(v);
+    }
+}
+
+// dw, db: the sums of all samples' pieces, 16 channels per workgroup, 16 lanes each
+__global__ __launch_bounds__(256) void param_grad_kernel(Args a, long items) {
+    __shared__ double2 red[16][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    double u = 0.0, v = 0.0;
+    if (c < a.C)
+        for (long i = r0; i < items; i += 16) {
+            const float2 s = a.bpart[i * a.C + c];
+            u += (double)s.x;
+            v += (double)s.y;
+        }
+    red[r0][threadIdx.x & 15] = make_double2(u, v);
+    __syncthreads();
+    if (r0 != 0 || c >= a.C) return;
+    for (int r = 1; r < 16; ++r) {
+        u += red[r][threadIdx.x].x;
+        v += red[r][threadIdx.x].y;
+    }
+    put_param(a.db, a.wtype, c, u);
+    put_param(a.dw, a.wtype, c, v);
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+struct Plan {
+    int threads, r;                             // resident: threads per sample and vectors per thread; 0: in pieces
+    int pc, rows_per, cc;
+};
+
+static int vec_of(const cmvae_group_norm& d, bool backward) {
+    const int full = d.dtype == CMVAE_F32 ? 4 : 8, es = d.dtype == CMVAE_F32 ? 4 : 2;
+    auto fits = [&](int v) {
+        auto ok = [&](const void* p, const int64_t* s) { return (uintptr_t)p % (v * es) == 0 && s[0] % v == 0 && s[1] % v == 0; };
+        const int64_t dense[2] = {0, 0};
+        return d.C % v == 0 && ok(d.x, d.x_stride) &&
+               (backward ? ok(d.dy, d.dy_stride) && ok(d.dx, dense) : ok(d.y, dense));
+    };
+    if (fits(full)) return full;
+    if (full == 8 && fits(2)) return 2;
+    return 1;
+}
+
+// Resident while a sample fits: 64 threads x 2 vectors, 256 x 2, 512 x 8, 1024 x 16 (forward; half in the backward,
+// which holds two tensors).
+static Plan plan_of(const cmvae_group_norm& d, int V, bool backward) {
+    Plan p = {0, 0, 1, d.P, 1};
+    const int CV = d.C / V;
+    const struct { int threads, r; } sizes[4] = {{64, 2}, {256, 2}, {512, 8}, {1024, backward ? 8 : 16}};
+    for (const auto& s : sizes) {
+        if (CV > s.threads || d.G > 1024) continue;
+        const int rows = s.threads / CV;
+        if ((long)rows * s.r >= d.P) {
+            p.threads = s.threads;
+            p.r = s.r;
+            return p;
+        }
+    }
+    p.cc = (CV + 255) / 256;
+    const int cw = CV < 256 ? CV : 256, rows = 256 / cw;
+    const long target = 2048, have = (long)d.N * p.cc;
+    long pc = (target + have - 1) / have;
+    const long most = (d.P + 4L * rows - 1) / (4L * rows);          // at least four pixels per thread
+    if (pc > most) pc = most;
+    if (pc < 1) pc = 1;
+    p.rows_per = (int)((d.P + pc - 1) / pc);
+    p.pc = (d.P + p.rows_per - 1) / p.rows_per;
+    return p;
+}
+
+static size_t ws_bytes(const cmvae_group_norm& d, const Plan& p, bool backward) {
+    const size_t nc = (size_t)d.N * p.pc * d.C;
+    if (!backward) return p.threads ? 0 : nc * sizeof(double2) + (size_t)d.N * d.G * sizeof(float4);
+    return nc * sizeof(float2) + 256 + (size_t)d.N * d.G * sizeof(float2);
+}
+
+template <typename K>
+static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a, void* stream, const char* what) {
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return set_error("%s: %s", what, hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, a);
+    return check_launch(what);
+}
+
+template <typename T, int V>
+static int run_fwd(Args a, const Plan& p, void* stream) {
+    if (p.threads) {
+        const size_t lds = (size_t)p.threads * V * sizeof(double2) + a.G * sizeof(float4);
+        const char* what = "group_norm fwd_resident_kernel";
+        switch (p.threads) {
+            case 64: return launch(fwd_resident_kernel<T, V, 64, 2>, a.N, 64, lds, a, stream, what);
+            case 256: return launch(fwd_resident_kernel<T, V, 256, 2>, a.N, 256, lds, a, stream, what);
+            case 512: return launch(fwd_resident_kernel<T, V, 512, 8>, a.N, 512, lds, a, stream, what);
+            default: return launch(fwd_resident_kernel<T, V, 1024, 16>, a.N, 1024, lds, a, stream, what);
+        }
+    }
+    const long blocks = (long)a.N * a.pc * a.cc;
+    if (int e = launch(fwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_sums_kernel")) return e;
+    if (int e = launch(fwd_finish_kernel, (long)a.N * a.G, 64, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
+    return launch(fwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_apply_kernel");
+}
+
+template <typename T, int V>
+static int run_bwd(Args a, const Plan& p, void* stream) {
+    int e;
+    if (p.threads) {
+        const size_t lds = (size_t)p.threads * V * sizeof(float2) + a.G * (sizeof(float4) + sizeof(float2));
+        const char* what = "group_norm bwd_resident_kernel";
+        switch (p.threads) {
+            case 64: e = launch(bwd_resident_kernel<T, V, 64, 2>, a.N, 64, lds, a, stream, what); break;
+            case 256: e = launch(bwd_resident_kernel<T, V, 256, 2>, a.N, 256, lds, a, stream, what); break;
+            case 512: e = launch(bwd_resident_kernel<T, V, 512, 8>, a.N, 512, lds, a, stream, what); break;
+            default: e = launch(bwd_resident_kernel<T, V, 1024, 8>, a.N, 1024, lds, a, stream, what);
+        }
+    } else {
+        const long blocks = (long)a.N * a.pc * a.cc;
+        if ((e = launch(bwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_sums_kernel"))) return e;
+        if ((e = launch(bwd_finish_kernel, (long)a.N * a.G, 64, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
+        e = launch(bwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_apply_kernel");
+    }
+    if (e || (!a.dw && !a.db)) return e;
+    hipLaunchKernelGGL(param_grad_kernel, dim3((a.C + 15) / 16), dim3(256), 0, (hipStream_t)stream, a, (long)a.N * a.pc);
+    return check_launch("group_norm param_grad_kernel");
+}
+
+template <typename T, int FULL>
+static int run(const Args& a, const Plan& p, int V, bool backward, void* stream) {
+    if (V == FULL) return backward ? run_bwd<T, FULL>(a, p, stream) : run_fwd<T, FULL>(a, p, stream);
+    if constexpr (FULL == 8) {
+        if (V == 2) return backward ? run_bwd<T, 2>(a, p, stream) : run_fwd<T, 2>(a, p, stream);
+    }
+    return backward ? run_bwd<T, 1>(a, p, stream) : run_fwd<T, 1>(a, p, stream);
+}
+
+static int check_desc(const char* who, const cmvae_group_norm* d) {
+    CMVAE_REQUIRE(d != nullptr, "%s: NULL descriptor", who);
+    CMVAE_REQUIRE(d->dtype >= CMVAE_F32 && d->dtype <= CMVAE_F16 && (d->wdtype == CMVAE_F32 || d->wdtype == d->dtype),
+                  "%s: dtype %d, parameters %d (fp32 or the data's)", who, d->dtype, d->wdtype);
+    CMVAE_REQUIRE(d->N >= 1 && d->P >= 1 && d->C >= 1 && d->G >= 1 && d->C % d->G == 0, "%s: N=%d P=%d C=%d groups=%d", who, d->N,
+                  d->P, d->C, d->G);
+    CMVAE_REQUIRE(d->act >= 0 && d->act <= 3, "%s: activation %d", who, d->act);
+    CMVAE_REQUIRE(d->eps >= 0.f && std::isfinite(d->eps), "%s: eps %g", who, (double)d->eps);
+    CMVAE_REQUIRE(d->x_stride[0] >= 0 && d->x_stride[1] >= 0, "%s: strides of x", who);
+    CMVAE_REQUIRE((long)d->N * d->G < (1L << 31) && d->C <= (1 << 24) && d->P <= (1 << 30), "%s: too large", who);
+    const uintptr_t es = d->dtype == CMVAE_F32 ? 4 : 2, ws = d->wdtype == CMVAE_F32 ? 4 : 2;
+    CMVAE_REQUIRE((((uintptr_t)d->x | (uintptr_t)d->y | (uintptr_t)d->dy | (uintptr_t)d->dx) & (es - 1)) == 0 &&
+                      (((uintptr_t)d->weight | (uintptr_t)d->bias | (uintptr_t)d->dweight | (uintptr_t)d->dbias) & (ws - 1)) == 0 &&
+                      ((uintptr_t)d->stats & 15) == 0,
+                  "%s: a tensor is not aligned", who);
+    return 0;
+}
+
+static Args args_of(const cmvae_group_norm& d, const Plan& p, int V) {
+    Args a = {};
+    a.x = d.x; a.dy = d.dy; a.w = d.weight; a.b = d.bias;
+    a.y = d.y; a.dx = d.dx; a.dw = d.dweight; a.db = d.dbias;
+    a.stats = (float4*)d.stats;
+    a.x_sn = d.x_stride[0]; a.x_sp = d.x_stride[1];
+    a.g_sn = d.dy_stride[0]; a.g_sp = d.dy_stride[1];
+    a.N = d.N; a.P = d.P; a.C = d.C; a.G = d.G; a.Cg = d.C / d.G; a.CV = d.C / V;
+    a.act = d.act; a.wtype = d.wdtype; a.eps = d.eps;
+    a.pc = p.pc; a.rows_per = p.rows_per; a.cc = p.cc;
+    return a;
+}
+
+static int enter(const char* who, const cmvae_group_norm* d, bool backward, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int e = check_desc(who, d)) return e;
+    if (backward)
+        CMVAE_REQUIRE(d->x && d->dy && d->dx && d->stats && d->dy_stride[0] >= 0 && d->dy_stride[1] >= 0, "%s: NULL tensor", who);
+    else
+        CMVAE_REQUIRE(d->x && d->y, "%s: NULL tensor", who);
+    const int V = vec_of(*d, backward);
+    const Plan p = plan_of(*d, V, backward);
+    const size_t need = ws_bytes(*d, p, backward);
+    CMVAE_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
+                  "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+    CMVAE_REQUIRE((long)d->N * p.pc * p.cc < (1L << 31), "%s: too large", who);
+    Args a = args_of(*d, p, V);
+    if (backward) {
+        a.bpart = (float2*)workspace;
+        a.means = (float2*)((char*)workspace + align_up((size_t)d->N * p.pc * d->C * sizeof(float2)));
+    } else if (!p.threads) {
+        a.part = (double2*)workspace;
+        if (!a.stats) a.stats = (float4*)(a.part + (size_t)d->N * p.pc * d->C);
+    }
+    switch (d->dtype) {
+        case CMVAE_F32: return run<float, 4>(a, p, V, backward, stream);
+        case CMVAE_BF16: return run<__bf16, 8>(a, p, V, backward, stream);
+        default: return run<_Float16, 8>(a, p, V, backward, stream);
+    }
+}
+
+}  // namespace gn
+}  // namespace cmvae
+
+using namespace cmvae;
+
+extern "C" size_t cmvae_group_norm_workspace_bytes(const cmvae_group_norm* d, int backward) {
+    cmvae::clear_stale_error();
+    if (gn::check_desc("cmvae_group_norm_workspace_bytes", d)) return 0;
+    const int V = gn::vec_of(*d, backward != 0);
+    return gn::ws_bytes(*d, gn::plan_of(*d, V, backward != 0), backward != 0);
+}
+
+extern "C" int cmvae_group_norm_fwd(const cmvae_group_norm* d, void* workspace, size_t workspace_bytes, void* stream) {
+    cmvae::clear_stale_error();
+    return gn::enter("cmvae_group_norm_fwd", d, false, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cmvae_group_norm_bwd(const cmvae_group_norm* d, void* workspace, size_t workspace_bytes, void* stream) {
+    cmvae::clear_stale_error();
+    return gn::enter("cmvae_group_norm_bwd", d, true, workspace, workspace_bytes, stream);
+}

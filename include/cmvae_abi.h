@@ -475,6 +475,25 @@ int cmvae_pool_bwd(const float* d_pool, const float* y, const float* scale, cons
                    const float* mean, const float* invstd, int n, int H, int W,
                    float* dybn, float* part, void* stream);
 
+/* ==== group norm with an activation on channels-last rows (statistics of one sample: no exchange between ranks, where
+ * BatchNorm2d over the meta-batch, omniglot/module.py:15-31, needs one per layer):
+ *   y = act((x - mean) rstd weight + bias), mean and biased variance per sample over P pixels x C / G channels.
+ * x, dy: [N, P, C] with strides {sample, pixel} in elements, channels adjacent; y, dx dense.  weight, bias, dweight,
+ * dbias [C] of fp32 or the data's dtype (wdtype), each may be NULL.  stats fp32 [N, G, 4] (mean in two parts, rstd, unused):
+ * written by the forward if not NULL, read by the backward.  act: 0 none, 1 ReLU, 2 ELU, 3 SiLU.  dtype as CMVAE_F32 ... */
+typedef struct cmvae_group_norm {
+    int32_t dtype, wdtype, act, N, P, C, G;
+    float eps;
+    const void *x, *weight, *bias, *dy;
+    int64_t x_stride[2], dy_stride[2];
+    void* y;
+    float* stats;
+    void *dx, *dweight, *dbias;
+} cmvae_group_norm;
+size_t cmvae_group_norm_workspace_bytes(const cmvae_group_norm* desc, int backward);     /* of the same descriptor */
+int cmvae_group_norm_fwd(const cmvae_group_norm* desc, void* workspace, size_t workspace_bytes, void* stream);
+int cmvae_group_norm_bwd(const cmvae_group_norm* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ==== EM seed stream (HOST function: every pointer is host memory, nothing is launched) ==================
  * The reference seeds the unsupervised EM with `np.random.choice(N, K, replace=False)` once per episode, in episode
  * order, from numpy's global generator (omniglot/model.py:351-356; mimgnet/model.py likewise).  This draws the
