@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import ops
-from ._lib import lib, check, SetAttnDesc
+from ._lib import lib, SetAttnDesc
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _p = ops._p
@@ -18,8 +18,8 @@ _p = ops._p
 
 def _rows16(t):
     """t with adjacent channels and rows that start at multiples of 16 bytes (a copy if it has not)."""
-    per = 16 // t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % per for s in t.stride()[:3]):
+    b, r, h, c = t.stride()
+    if c != 1 or t.data_ptr() % 16 or (b | r | h) % (16 // t.element_size()):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -51,55 +51,51 @@ def _check(q, k, v, scale, q_len, k_len):
             ops.check_index_range(t, S + 1, n)
 
 
-def _desc(q, k, v, scale, causal, q_len, k_len, residual):
-    d = SetAttnDesc()
-    d.dtype = DTYPES[q.dtype]
-    d.B, d.Sq, d.H, d.D = q.shape
-    d.Sk, d.Hkv = k.shape[1:3]
-    d.causal, d.residual, d.scale = int(causal), int(residual), scale
-    d.q, d.k, d.v, d.q_len, d.k_len = _p(q), _p(k), _p(v), _p(q_len), _p(k_len)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    return d
+def _desc(q, k, v, scale, causal, q_len, k_len, residual, do=None):
+    B, Sq, H, D = q.shape
+    return SetAttnDesc(DTYPES[q.dtype], B, Sq, k.shape[1], H, k.shape[2], D, causal, residual, scale, q.data_ptr(),
+                       k.data_ptr(), v.data_ptr(), _p(do), q.stride()[:3], k.stride()[:3], v.stride()[:3],
+                       do.stride()[:3] if do is not None else (0, 0, 0), _p(q_len), _p(k_len))
 
 
 def _workspace(d, backward, device):
     # from the caching allocator, per call: a captured graph owns its own
     n = lib.cmvae_set_attention_workspace_bytes(ctypes.byref(d), backward)
-    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return ws, n
 
 
 def set_attention_fwd(q, k, v, scale, causal, q_len, k_len, residual, save):
     """(o, attn, lse) of one call; attn and lse are None unless `save` (attn: o without the residual)."""
     B, Sq, H, D = q.shape
-    o = torch.empty(B, Sq, H, D, device=q.device, dtype=q.dtype)
+    dev = q.device
+    o = torch.empty((B, Sq, H, D), device=dev, dtype=q.dtype)
     attn = (torch.empty_like(o) if residual else o) if save else None
-    lse = torch.empty(B, H, Sq, device=q.device, dtype=torch.float32) if save else None
+    lse = torch.empty((B, H, Sq), device=dev, dtype=torch.float32) if save else None
     if o.numel() == 0:
         return o, attn, lse
     d = _desc(q, k, v, scale, causal, q_len, k_len, residual)
-    d.o, d.attn, d.lse = _p(o), (_p(attn) if residual else None), _p(lse)
-    with torch.cuda.device(q.device):
-        ws, n = _workspace(d, 0, q.device)
-        check(lib.cmvae_set_attention_fwd(ctypes.byref(d), _p(ws), n, ops._stream()), 'cmvae_set_attention_fwd')
+    d.o, d.attn, d.lse = o.data_ptr(), (_p(attn) if residual else None), _p(lse)
+    ws, n = _workspace(d, 0, dev)
+    ops._call('cmvae_set_attention_fwd', lib.cmvae_set_attention_fwd, dev, ctypes.byref(d), _p(ws), n)
     return o, attn, lse
 
 
 def set_attention_bwd(q, k, v, attn, lse, do, scale, causal, q_len, k_len, residual):
     """(dq, dk, dv) from the tensors `set_attention_fwd` was given and saved."""
-    B, Sq, H, D = q.shape
-    dq = torch.empty(B, Sq, H, D, device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
+    dev = q.device
+    dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    dk = torch.empty(k.shape, device=dev, dtype=q.dtype)
+    dv = torch.empty(k.shape, device=dev, dtype=q.dtype)
     if dq.numel() == 0:
         return dq, dk.zero_(), dv.zero_()
     delta = torch.empty_like(lse)
-    d = _desc(q, k, v, scale, causal, q_len, k_len, residual)
     do = _rows16(do)
-    d.dO, d.dO_stride[:] = _p(do), do.stride()[:3]
-    d.o = d.attn = _p(attn)
-    d.lse, d.delta, d.dq, d.dk, d.dv = _p(lse), _p(delta), _p(dq), _p(dk), _p(dv)
-    with torch.cuda.device(q.device):
-        ws, n = _workspace(d, 1, q.device)
-        check(lib.cmvae_set_attention_bwd(ctypes.byref(d), _p(ws), n, ops._stream()), 'cmvae_set_attention_bwd')
+    d = _desc(q, k, v, scale, causal, q_len, k_len, residual, do)
+    d.o = d.attn = attn.data_ptr()
+    d.lse, d.delta, d.dq, d.dk, d.dv = lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    ws, n = _workspace(d, 1, dev)
+    ops._call('cmvae_set_attention_bwd', lib.cmvae_set_attention_bwd, dev, ctypes.byref(d), _p(ws), n)
     return dq, dk, dv
 
 

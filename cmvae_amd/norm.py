@@ -9,7 +9,7 @@ import math
 import torch
 
 from . import ops
-from ._lib import lib, check, GroupNormDesc
+from ._lib import lib, GroupNormDesc
 from .attention import DTYPES
 
 ACT = {None: 0, 'none': 0, 'relu': 1, 'elu': 2, 'silu': 3}
@@ -18,8 +18,9 @@ _p = ops._p
 
 def _rows(x):
     """[N, ..., C] -> [N, P, C] with adjacent channels (a copy where strides do not allow it)."""
-    x3 = x.reshape(x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1])
-    return x3 if x3.stride(2) == 1 else x3.contiguous()
+    if x.dim() != 3:
+        x = x.reshape(x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1])
+    return x if x.stride(2) == 1 else x.contiguous()
 
 
 def _check(x, groups, weight, bias, eps, act):
@@ -46,50 +47,46 @@ def _check(x, groups, weight, bias, eps, act):
 
 
 def _strides(x3):
-    return [x3.stride(i) if x3.shape[i] > 1 else 0 for i in (0, 1)]
+    n, p, _ = x3.stride()
+    return n if x3.shape[0] > 1 else 0, p if x3.shape[1] > 1 else 0
 
 
-def _desc(x3, groups, weight, bias, eps, act):
-    d = GroupNormDesc()
-    d.dtype, d.act, d.eps = DTYPES[x3.dtype], act, eps
+def _desc(x3, groups, weight, bias, eps, act, dy3=None):
     ref = weight if weight is not None else bias
-    d.wdtype = DTYPES[ref.dtype] if ref is not None else 0
-    d.N, d.P, d.C = x3.shape
-    d.G = groups
-    d.x, d.x_stride[:] = _p(x3), _strides(x3)
-    d.weight, d.bias = _p(weight), _p(bias)
-    return d
+    return GroupNormDesc(DTYPES[x3.dtype], DTYPES[ref.dtype] if ref is not None else 0, act, *x3.shape, groups, eps,
+                         x3.data_ptr(), _p(weight), _p(bias), _p(dy3), _strides(x3),
+                         _strides(dy3) if dy3 is not None else (0, 0))
 
 
-def _run(name, d, backward, device):
-    with torch.cuda.device(device):
-        n = lib.cmvae_group_norm_workspace_bytes(ctypes.byref(d), backward)
-        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        check(getattr(lib, name)(ctypes.byref(d), _p(ws), n, ops._stream()), name)
+def _run(name, fn, d, backward, device):
+    n = lib.cmvae_group_norm_workspace_bytes(ctypes.byref(d), backward)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    ops._call(name, fn, device, ctypes.byref(d), _p(ws), n)
 
 
 def group_norm_fwd(x3, groups, weight, bias, eps, act, save):
     """(y [N, P, C], stats [N, groups, 4] or None); stats: mean in two parts, 1 / deviation."""
-    y = torch.empty(x3.shape, device=x3.device, dtype=x3.dtype)
-    stats = torch.empty(x3.shape[0], groups, 4, device=x3.device, dtype=torch.float32) if save else None
+    dev = x3.device
+    y = torch.empty(x3.shape, device=dev, dtype=x3.dtype)
+    stats = torch.empty((x3.shape[0], groups, 4), device=dev, dtype=torch.float32) if save else None
     if y.numel():
         d = _desc(x3, groups, weight, bias, eps, act)
-        d.y, d.stats = _p(y), _p(stats)
-        _run('cmvae_group_norm_fwd', d, 0, x3.device)
+        d.y, d.stats = y.data_ptr(), _p(stats)
+        _run('cmvae_group_norm_fwd', lib.cmvae_group_norm_fwd, d, 0, dev)
     return y, stats
 
 
 def group_norm_bwd(x3, dy3, groups, weight, bias, stats, eps, act, need_params):
     """(dx, dweight, dbias) of one `group_norm_fwd` that saved its stats."""
-    dx = torch.empty(x3.shape, device=x3.device, dtype=x3.dtype)
+    dev = x3.device
+    dx = torch.empty(x3.shape, device=dev, dtype=x3.dtype)
     dw = torch.empty_like(weight) if weight is not None and need_params else None
     db = torch.empty_like(bias) if bias is not None and need_params else None
     if dx.numel() == 0:
         return dx, (None if dw is None else dw.zero_()), (None if db is None else db.zero_())
-    d = _desc(x3, groups, weight, bias, eps, act)
-    d.dy, d.dy_stride[:] = _p(dy3), _strides(dy3)
-    d.stats, d.dx, d.dweight, d.dbias = _p(stats), _p(dx), _p(dw), _p(db)
-    _run('cmvae_group_norm_bwd', d, 1, x3.device)
+    d = _desc(x3, groups, weight, bias, eps, act, dy3)
+    d.stats, d.dx, d.dweight, d.dbias = stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db)
+    _run('cmvae_group_norm_bwd', lib.cmvae_group_norm_bwd, d, 1, dev)
     return dx, dw, db
 
 
@@ -104,7 +101,7 @@ class _GroupNormAct(torch.autograd.Function):
         if save:
             ctx.args = (groups, eps, act, x.shape)
             ctx.save_for_backward(x3, weight, bias, stats)
-        return y.view(x.shape)
+        return y if x.dim() == 3 else y.view(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -113,7 +110,7 @@ class _GroupNormAct(torch.autograd.Function):
         groups, eps, act, shape = ctx.args
         dx, dw, db = group_norm_bwd(x3, _rows(dy), groups, weight, bias, stats, eps, act,
                                     ctx.needs_input_grad[2] or ctx.needs_input_grad[3])
-        return dx.view(shape), None, dw, db, None, None
+        return dx if len(shape) == 3 else dx.view(shape), None, dw, db, None, None
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act=None):

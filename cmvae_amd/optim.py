@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import ops
-from ._lib import lib, check
+from ._lib import lib
 from .attention import DTYPES
 
 BLOCK = 256                    # values that share a scale; every tensor's states start at a multiple of it
@@ -59,30 +59,28 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, scales=None, step=1, lr=1e-3,
     params, grads = list(params), list(grads)
     if len(params) != len(grads):
         raise RuntimeError('cmvae_amd adamw: %d parameters and %d gradients' % (len(params), len(grads)))
-    flat, at, seen, done, keep = [], 0, set(), [], []
+    flat, at, done, keep = [], 0, [], []
     for p, g in zip(params, grads):
         n = p.numel()
         here, at = at, at + (n + BLOCK - 1) // BLOCK * BLOCK
         if g is None:
             continue
-        code = DTYPES.get(p.dtype)
-        if code is None or g.dtype != p.dtype or p.device != dev or g.device != dev or g.shape != p.shape:
+        dt, st = p.dtype, p.stride()
+        if dt not in DTYPES or g.dtype is not dt or p.device != dev or g.device != dev or g.shape != p.shape:
             raise RuntimeError('cmvae_amd adamw: a parameter %s %s on %s with a gradient %s %s on %s (float32, bfloat16 or '
                                'float16, alike, on the states\' device)' % (p.dtype, tuple(p.shape), p.device, g.dtype,
                                                                             tuple(g.shape), g.device))
         if not p.is_contiguous() and not (p.dim() == 4 and p.is_contiguous(memory_format=torch.channels_last)):
             raise RuntimeError('cmvae_amd adamw: a parameter of shape %s has strides %s: it must be dense'
-                               % (tuple(p.shape), p.stride()))
-        if g.stride() != p.stride():
+                               % (tuple(p.shape), st))
+        if g.stride() != st:
             g = torch.empty_like(p).copy_(g)
             keep.append(g)
-        ptr = p.data_ptr()
         if n:
-            if ptr in seen:
-                raise RuntimeError('cmvae_amd adamw: a parameter appears twice')
-            seen.add(ptr)
-        done.append(p)
-        flat += (ptr, g.data_ptr(), n, here, code)
+            done.append(p)
+            flat += (p.data_ptr(), g.data_ptr(), n, here, DTYPES[dt])
+    if len(set(flat[::5])) != len(done):
+        raise RuntimeError('cmvae_amd adamw: a parameter appears twice')
     if at != length:
         raise RuntimeError('cmvae_amd adamw: the parameters take %d state values, the states hold %d' % (at, length))
     step_dev = None
@@ -92,10 +90,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, scales=None, step=1, lr=1e-3,
         step, step_dev = 0, step
     if not done:
         return
-    with torch.cuda.device(dev):
-        check(lib.cmvae_adamw_step((ctypes.c_int64 * len(flat))(*flat), len(done), bits, _p(exp_avg), _p(exp_avg_sq),
-                                   _p(scales), length, int(step), _p(step_dev), lr, betas[0], betas[1], eps, weight_decay,
-                                   ops._stream()), 'cmvae_adamw_step')
+    ops._call('cmvae_adamw_step', lib.cmvae_adamw_step, dev, (ctypes.c_int64 * len(flat))(*flat), len(done), bits,
+              exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _p(scales), length, int(step), _p(step_dev), lr, betas[0], betas[1],
+              eps, weight_decay)
     torch.autograd.graph.increment_version(done)
 
 
@@ -105,9 +102,8 @@ def adamw_state_values(exp_avg, exp_avg_sq, scales):
     if bits == 32:
         raise RuntimeError('cmvae_amd adamw: states in 32 bits are their values')
     m, v = (torch.empty(n, device=dev, dtype=torch.float32) for _ in range(2))
-    with torch.cuda.device(dev):
-        check(lib.cmvae_adamw_state_values(_p(exp_avg), _p(exp_avg_sq), _p(scales), n, _p(m), _p(v), ops._stream()),
-              'cmvae_adamw_state_values')
+    ops._call('cmvae_adamw_state_values', lib.cmvae_adamw_state_values, dev, _p(exp_avg), _p(exp_avg_sq), _p(scales), n, _p(m),
+              _p(v))
     return m, v
 
 
