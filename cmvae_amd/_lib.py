@@ -8,6 +8,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('CMVAE_HIP_LIB') or os.path.join(_HERE, 'libcmvae_hip.so')      # override: profiling builds
+TORCH_OPS_PATH = os.path.join(_HERE, '_torch_ops.so')
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -204,7 +205,18 @@ def _load():
     return lib
 
 
+def _load_torch_ops():
+    """torch.ops.cmvae_amd.{set_attention, group_norm_act, adamw_step, adamw_state_values}: bound in C++
+    (cmvae_amd/csrc/torch_ops.cpp) to the entry points of the library above."""
+    import torch
+    if not os.path.exists(TORCH_OPS_PATH):
+        raise ImportError('cmvae_amd: %s not found. Build it with `make -C cmvae_amd/csrc`.' % TORCH_OPS_PATH)
+    torch.ops.load_library(TORCH_OPS_PATH)
+    torch.ops.cmvae_amd._use_library(LIB_PATH)
+
+
 lib = _load()
+_load_torch_ops()
 
 
 def check(rc, what=''):

@@ -41,7 +41,7 @@ struct Args {
     float *lse, *delta, *part, *part_ml;
     const int *q_len, *k_len;
     long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, g_sb, g_ss, g_sh;   // strides in elements
-    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, split_tiles, ntiles;
+    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, split_tiles, ntiles, sg;
     float scale, c;                                                                // c = scale * log2(e)
 };
 
@@ -280,7 +280,7 @@ __device__ __forceinline__ void span(const Args& a, int r0, int r1, int& lo, int
 // NW waves of 32 rows; keys in tiles of KT through LDS, two buffers.  Running maximum m (log2 units) and sum l per row.
 // nsplit > 1: a workgroup covers split_tiles tiles and leaves (acc, m, l) for the joining kernel.
 template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = KT * pitch<T, D>();
     const Place pl = place(a, a.causal);
@@ -403,31 +403,54 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
         }
 }
 
-// joins the splits of a row: D / 4 lanes per row
+// Joins the splits of a row: D / 4 lanes per row times SG groups that share its splits out (SG from the host: few rows of
+// many splits would otherwise be a long walk on a handful of lanes; 16 rows of 50 splits took 24 us that way).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
     constexpr int LPR = D / 4;
+    __shared__ float sm[256], sl[256];
+    __shared__ f32x4 so[256];
     const long rows = (long)a.B * a.Hkv * a.R;
-    const long row = (blockIdx.x * 256L + threadIdx.x) / LPR;
-    const int d4 = threadIdx.x % LPR;
+    const int rpb = 256 / LPR / a.sg, lr = (int)threadIdx.x / (LPR * a.sg);
+    const int d4 = threadIdx.x % LPR, sg = (int)threadIdx.x / LPR % a.sg;
+    const long row = (long)blockIdx.x * rpb + lr;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (row < rows) {
+        for (int s = sg; s < a.nsplit; s += a.sg) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
+        const float mu = m == -INFINITY ? 0.f : m;
+        for (int s = sg; s < a.nsplit; s += a.sg) {
+            const long at = s * rows + row;
+            const float wgt = exp2_raw(a.part_ml[at * 2] - mu);
+            l = fmaf(wgt, a.part_ml[at * 2 + 1], l);
+            const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + at * D + d4 * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(wgt, p[j], o[j]);
+        }
+    }
+    if (a.sg > 1) {
+        sm[threadIdx.x] = m;
+        sl[threadIdx.x] = l;
+        so[threadIdx.x] = o;
+        __syncthreads();
+        if (sg != 0) return;
+        for (int i = 1; i < a.sg; ++i) m = fmaxf(m, sm[threadIdx.x + i * LPR]);
+        const float mu = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < a.sg; ++i) {
+            const float wgt = exp2_raw(sm[threadIdx.x + i * LPR] - mu);
+            l = fmaf(wgt, sl[threadIdx.x + i * LPR], l);
+            const f32x4 p = so[threadIdx.x + i * LPR];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(wgt, p[j], o[j]);
+        }
+    }
     if (row >= rows) return;
     const int b = (int)(row / ((long)a.H * a.Sq));
     const int rest = (int)(row - (long)b * a.H * a.Sq), head = rest / a.Sq, pos = rest - head * a.Sq;
     int ql, kl;
     lens(a, b, ql, kl);
-    float m = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_ml[(s * rows + row) * 2]);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const long at = s * rows + row;
-        const float wgt = exp2_raw(a.part_ml[at * 2] - mu);
-        l = fmaf(wgt, a.part_ml[at * 2 + 1], l);
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + at * D + d4 * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(wgt, p[j], o[j]);
-    }
     const bool ok = pos < ql && l != 0.f;
     if (d4 == 0 && a.lse) a.lse[row] = ok ? m - p_shift<T>() + log2f(l) : INFINITY;
     const float inv = ok ? 1.f / l : 0.f;
@@ -439,10 +462,27 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
     store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
 }
 
+// sum over the splits of the 4 values at `e` of n4, shared out over SG groups of 256 / SG threads; true in the group that
+// has the sum
+__device__ __forceinline__ bool join_sum(const Args& a, const float* part, long n4, long e, int sg, f32x4& x) {
+    __shared__ f32x4 red[256];
+    x = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int per = 256 / a.sg;
+    if (e < n4)
+        for (int s = sg; s < a.nsplit; s += a.sg) x += reinterpret_cast<const f32x4*>(part)[s * n4 + e];
+    if (a.sg == 1) return true;
+    __syncthreads();
+    red[threadIdx.x] = x;
+    __syncthreads();
+    if (sg != 0) return false;
+    for (int i = 1; i < a.sg; ++i) x += red[threadIdx.x + i * per];
+    return true;
+}
+
 // ------------------------------------------------------------------------------------------------ backward, query side
 // The forward's shape; delta_i from the saved o, kept for the key side.
 template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, 2) void dq_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = KT * pitch<T, D>();
     const Place pl = place(a, a.causal);
@@ -543,15 +583,15 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
     constexpr int LPR = D / 4;
     const long rows = (long)a.B * a.Hkv * a.R;
-    const long row = (blockIdx.x * 256L + threadIdx.x) / LPR;
-    const int d4 = threadIdx.x % LPR;
-    if (row >= rows) return;
+    const int per = 256 / a.sg, sg = (int)threadIdx.x / per;
+    const long e = (long)blockIdx.x * per + threadIdx.x - sg * per, row = e / LPR;
+    const int d4 = (int)(e - row * LPR);
+    f32x4 o;
+    if (!join_sum(a, a.part, rows * LPR, e, sg, o) || row >= rows) return;
     const int b = (int)(row / ((long)a.H * a.Sq));
     const int rest = (int)(row - (long)b * a.H * a.Sq), head = rest / a.Sq, pos = rest - head * a.Sq;
     int ql, kl;
     lens(a, b, ql, kl);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) o += *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * D + d4 * 4);
     const long es = sizeof(T);
     if (a.residual && pos < ql) o += load4<T>(a.doo + (b * a.g_sb + pos * a.g_ss + head * a.g_sh + d4 * 4) * es);
     store4<T>(a.dq + ((((long)b * a.Sq + pos) * a.H + head) * D + d4 * 4) * es, o[0], o[1], o[2], o[3]);
@@ -560,7 +600,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------ backward, key side
 // NW waves of 32 keys; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
 template <typename T, int D, int NW, int RT>
-__global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = RT * pitch<T, D>(), BUF = 2 * TB + RT * 8;
     const Place pl = place(a, false);
@@ -688,14 +728,12 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void dkv_join_kernel(Args a, long n4) {
-    const long e = blockIdx.x * 256L + threadIdx.x;
-    if (e >= n4) return;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-    const f32x4* p = reinterpret_cast<const f32x4*>(a.part);
-    for (int s = 0; s < a.nsplit; ++s) {
-        x += p[s * n4 + e];
-        y += p[(a.nsplit + s) * n4 + e];
-    }
+    const int per = 256 / a.sg, sg = (int)threadIdx.x / per;
+    const long e = (long)blockIdx.x * per + threadIdx.x - sg * per;
+    f32x4 x, y;
+    const bool mine = join_sum(a, a.part, n4, e, sg, x);
+    join_sum(a, a.part + (size_t)a.nsplit * n4 * 4, n4, e, sg, y);
+    if (!mine || e >= n4) return;
     store4<T>(a.dk + e * 4 * sizeof(T), x[0], x[1], x[2], x[3]);
     store4<T>(a.dv + e * 4 * sizeof(T), y[0], y[1], y[2], y[3]);
 }
@@ -769,6 +807,13 @@ static void use(Args& a, const Plan& p) {
     a.split_tiles = p.split_tiles;
 }
 
+// groups that share out the splits of one value in a joining kernel of n4 x 4 values: until the launch fills the card
+static int join_groups(int nsplit, long n4, int most) {
+    int sg = 1;
+    while (sg < most && 2 * sg <= nsplit && n4 * sg < 256L * 1024) sg *= 2;
+    return sg;
+}
+
 template <typename T, int D>
 static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
     constexpr int T4 = sizeof(T) * D <= 256 ? 64 : 32;
@@ -780,7 +825,8 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
     int e = z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
                         : launch(fwd_kernel<T, D, 1, 32>, blocks, 64, z.f.lds, a, stream, "set_attention fwd_kernel");
     if (e || a.nsplit == 1) return e;
-    return launch(fwd_join_kernel<T, D>, (rows * (D / 4) + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
+    a.sg = join_groups(a.nsplit, rows * (D / 4), 256 / (D / 4));
+    return launch(fwd_join_kernel<T, D>, (rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
 }
 
 template <typename T, int D>
@@ -793,16 +839,19 @@ static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
     int e = z.q.nw == 4 ? launch(dq_kernel<T, D, 4, T4>, blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
                         : launch(dq_kernel<T, D, 1, 32>, blocks, 64, z.q.lds, a, stream, "set_attention dq_kernel");
     if (e) return e;
-    if (a.nsplit > 1 &&
-        (e = launch(dq_join_kernel<T, D>, (rows * (D / 4) + 255) / 256, 256, 0, a, stream, "set_attention dq_join_kernel")))
-        return e;
+    if (a.nsplit > 1) {
+        a.sg = join_groups(a.nsplit, rows * (D / 4), 16);
+        if ((e = launch(dq_join_kernel<T, D>, (rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dq_join_kernel")))
+            return e;
+    }
     use(a, z.k);
     blocks = nbh * a.ntiles * a.nsplit;
     e = z.k.nw == 4 ? launch(dkv_kernel<T, D, 4, T4>, blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
                     : launch(dkv_kernel<T, D, 1, 32>, blocks, 64, z.k.lds, a, stream, "set_attention dkv_kernel");
     if (e || a.nsplit == 1) return e;
     const long n4 = keys * D / 4;
-    hipLaunchKernelGGL(dkv_join_kernel<T>, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a, n4);
+    a.sg = join_groups(a.nsplit, n4, 16);
+    hipLaunchKernelGGL(dkv_join_kernel<T>, dim3((unsigned)((n4 * a.sg + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a, n4);
     return check_launch("set_attention dkv_join_kernel");
 }
 

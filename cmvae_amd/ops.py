@@ -25,23 +25,6 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
-
-def _call(name, fn, device, *args):
-    """fn(*args, stream) on `device`, whose current stream is passed: the entry point launches there whatever device is
-    the current one.  (The stream's raw handle costs 0.1 us; `torch.cuda.current_stream()` 3 us, 15 us in autograd's
-    own thread, which wakes with cold caches for every backward pass.)"""
-    i = device.index
-    if i == _current_device():
-        rc = fn(*args, _raw_stream(i))
-    else:
-        with torch.cuda.device(i):
-            rc = fn(*args, _raw_stream(i))
-    if rc:
-        check(rc, name)
-
-
 def _req(t, name, dtype=torch.float32, shape=None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError('cmvae_amd: %s must be a tensor on the MI355X device (no CPU path exists)' % name)

@@ -423,4 +423,6 @@ def _decoder_bce(h_rec, target, M, training, params, running, eps, momentum):
 
 _d.impl('encode_images', _encode_images, 'CompositeImplicitAutograd')
 _d.impl('decoder_bce', _decoder_bce, 'CompositeImplicitAutograd')
-REGISTERED = REGISTERED + ('encode_images', 'decoder_bce')
+# bound in C++, with their autograd nodes (cmvae_amd/csrc/torch_ops.cpp); called by attention.py, norm.py and optim.py
+REGISTERED = REGISTERED + ('encode_images', 'decoder_bce', 'set_attention', 'group_norm_act', 'adamw_step',
+                           'adamw_state_values')
