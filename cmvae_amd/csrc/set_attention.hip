@@ -5,9 +5,9 @@
 //   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i . v_j - delta_i),   delta_i = do_i . sum_j p_ij v_j
 //   dq_i = scale sum_j ds_ij k_j (+ do_i if residual),   dk_j = scale sum_i ds_ij q_i
 //
-// The G = H / Hkv query heads that share a key head are one list of R = G * Sq rows (row r = head r / Sq, position
-// r % Sq), so a tile of keys is read once for all of them and the gradients of shared heads are summed in registers, in
-// a fixed order.
+// The G = H / Hkv query heads that share a key head are one list of rows — the G * q_len rows that count (row r = head
+// r / q_len, position r % q_len), then the others, which only get zeros — so a tile of keys is read once for all of them and
+// the gradients of shared heads are summed in registers, in a fixed order.
 //
 // Every product is a 32 x 32 matrix instruction with the contraction's second factor in registers.  The forward and the dq
 // kernel hold 32 query rows per wave and form S^T (keys x queries): a lane then has 16 keys of ONE query, so the softmax
@@ -41,7 +41,7 @@ struct Args {
     float *lse, *delta, *part, *part_ml;
     const int *q_len, *k_len;
     long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, g_sb, g_ss, g_sh;   // strides in elements
-    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, split_tiles, ntiles, sg;
+    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, ntiles, sg, fold;
     float scale, c;                                                                // c = scale * log2(e)
 };
 
@@ -218,15 +218,15 @@ struct Stage {
             if (row < end) x[i] = *reinterpret_cast<const u32x4*>(base + row * stride_bytes + (id % CPR) * 16);
         }
     }
-    // query rows r0 .. of a key head's list: (head, position) = divmod(r, Sq); positions from q_end on are zeros
-    __device__ __forceinline__ void load_rows(const char* base, long ss, long sh, int r0, int R, int Sq, int q_end) {
+    // query rows r0 .. of a key head's list: (head, position) = divmod(r, ql); rows from `end` = G ql on are zeros
+    __device__ __forceinline__ void load_rows(const char* base, long ss, long sh, int r0, int end, int ql) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = i * THREADS + threadIdx.x, r = r0 + id / CPR;
             x[i] = u32x4{0, 0, 0, 0};
-            if (r < R) {
-                const int g = r / Sq, pos = r - g * Sq;
-                if (pos < q_end) x[i] = *reinterpret_cast<const u32x4*>(base + pos * ss + g * sh + (id % CPR) * 16);
+            if (r < end) {
+                const int g = r / ql, pos = r - g * ql;
+                x[i] = *reinterpret_cast<const u32x4*>(base + pos * ss + g * sh + (id % CPR) * 16);
             }
         }
     }
@@ -239,24 +239,6 @@ struct Stage {
     }
 };
 
-struct Place {           // what a workgroup works on
-    int b, kh, tile, split;
-};
-// (batch, key head) runs fastest: with a multiple of 8 of them each stays on one XCD, whose L2 then holds its keys
-__device__ __forceinline__ Place place(const Args& a, bool last_first) {
-    const int nbh = a.B * a.Hkv;
-    int id = blockIdx.x;
-    Place p;
-    const int bh = id % nbh;
-    id /= nbh;
-    p.split = id % a.nsplit;
-    id /= a.nsplit;
-    p.tile = last_first ? a.ntiles - 1 - id : id;
-    p.b = bh / a.Hkv;
-    p.kh = bh - p.b * a.Hkv;
-    return p;
-}
-
 __device__ __forceinline__ void lens(const Args& a, int b, int& ql, int& kl) {
     ql = a.Sq;
     kl = a.Sk;
@@ -264,16 +246,98 @@ __device__ __forceinline__ void lens(const Args& a, int b, int& ql, int& kl) {
     if (a.k_len) kl = min(max(a.k_len[b], 0), a.Sk);
 }
 
-// positions [lo, hi] that the rows r0 .. r1 - 1 of a key head's list cover
-__device__ __forceinline__ void span(const Args& a, int r0, int r1, int& lo, int& hi) {
-    const int g0 = r0 / a.Sq, g1 = (r1 - 1) / a.Sq;
-    if (g0 == g1) {
-        lo = r0 - g0 * a.Sq;
-        hi = r1 - 1 - g0 * a.Sq;
-    } else {
-        lo = 0;
-        hi = a.Sq - 1;
+struct Place {           // what a workgroup works on
+    int b, kh, tile, split, ql, kl;
+};
+
+// Which piece of work a workgroup takes.  A compute unit holds few workgroups, each of them long, so what matters is that its
+// sum is near the others'.
+//   Lengths given (and up to 64 batch entries): every workgroup ranks the entries by the length that its side walks, one lane
+//   per entry, and the tiles are dealt longest first, those without a valid row last.
+//   Otherwise: (batch, key head) runs fastest — with a multiple of 8 of them each stays on one XCD, whose L2 then holds its
+//   keys — and the causal order's longest tiles come first.
+// With one to two workgroups per compute unit the second ones are dealt shortest first: each joins a long one.
+// Measured on 16 padded sets of 383 to 1531 rows, fp32, against plain order: forward 371 -> @F@ us, dq 522 -> @Q@, dk and dv
+// 690 -> @K@.
+template <int ROWS, bool KEYS>
+__device__ __forceinline__ Place place(const Args& a) {
+    Place p;
+    int id = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    // one to two workgroups per compute unit, both resident: the second ones are dealt shortest first, each joins a long one
+    auto fold = [&](int jobs) {
+        if (jobs > a.fold && jobs <= 2 * a.fold && id >= a.fold && id < jobs) id = a.fold + jobs - 1 - id;
+    };
+    // the causal order's longest tiles first: of a list of n tiles that runs through G heads, every head's last one, then every
+    // head's last but one ...
+    auto longest_first = [&](int i, int n) {
+        if (!a.causal || KEYS) return i;
+        const int per = n / a.G, more = n - per * a.G;             // the first `more` heads have per + 1 tiles
+        int round = i / a.G, g = i - round * a.G;
+        return (g + 1) * per + min(g + 1, more) - 1 - round;
+    };
+    if ((a.q_len || a.k_len) && a.B <= 64) {
+        int ql, kl, nt = 0, w = 0;
+        lens(a, lane < a.B ? lane : 0, ql, kl);
+        if (lane < a.B) {
+            nt = KEYS ? (kl + ROWS - 1) / ROWS : (a.G * ql + ROWS - 1) / ROWS;
+            w = KEYS ? ql : kl;
+        }
+        int start = 0, zeros = 0, total = 0;               // tiles before this lane's entry's, tiles without a row before them
+        for (int i = 0; i < a.B; ++i) {
+            const int wi = __builtin_amdgcn_readlane(w, i), ni = __builtin_amdgcn_readlane(nt, i);
+            start += wi > w || (wi == w && i < lane) ? ni : 0;
+            zeros += i < lane ? a.ntiles - ni : 0;
+            total += ni;
+        }
+        fold(total * a.Hkv * a.nsplit);
+        p.split = id % a.nsplit;
+        id /= a.nsplit;
+        p.kh = id % a.Hkv;
+        id /= a.Hkv;
+        const bool some = id < total;
+        const int at = some ? id - start : id - total - zeros;
+        const unsigned long long mine = __ballot(lane < a.B && at >= 0 && at < (some ? nt : a.ntiles - nt));
+        p.b = __ffsll((long long)mine) - 1;
+        const int t = __builtin_amdgcn_readlane(at, p.b), n = __builtin_amdgcn_readlane(nt, p.b);
+        p.tile = some ? longest_first(t, n) : n + t;
+        p.ql = __builtin_amdgcn_readlane(ql, p.b);
+        p.kl = __builtin_amdgcn_readlane(kl, p.b);
+        return p;
     }
+    const int nbh = a.B * a.Hkv;
+    if (a.causal) fold(nbh * a.ntiles * a.nsplit);
+    const int bh = id % nbh;
+    id /= nbh;
+    p.split = id % a.nsplit;
+    id /= a.nsplit;
+    p.tile = longest_first(id, a.ntiles);
+    p.b = bh / a.Hkv;
+    p.kh = bh - p.b * a.Hkv;
+    lens(a, p.b, p.ql, p.kl);
+    return p;
+}
+
+// row r of a key head's list: its head in the group and its position; whether it counts
+struct Row {
+    int g, pos;
+    bool ok;
+};
+__device__ __forceinline__ Row row_of(const Args& a, int ql, int r) {
+    const int valid = a.G * ql;
+    Row w;
+    w.ok = r < valid;
+    const int x = w.ok ? r : r - valid, n = w.ok ? ql : a.Sq - ql;
+    w.g = n > 0 ? x / n : 0;
+    w.pos = x - w.g * n + (w.ok ? 0 : ql);
+    return w;
+}
+
+// positions [lo, hi] that the valid rows r0 .. r1 - 1 of a key head's list cover
+__device__ __forceinline__ void span(int ql, int r0, int r1, int& lo, int& hi) {
+    const int g0 = r0 / ql, g1 = (r1 - 1) / ql;
+    lo = g0 == g1 ? r0 - g0 * ql : 0;
+    hi = g0 == g1 ? r1 - 1 - g0 * ql : ql - 1;
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -283,22 +347,25 @@ template <typename T, int D, int NW, int KT>
 __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = KT * pitch<T, D>();
-    const Place pl = place(a, a.causal);
+    const Place pl = place<NW * 32, false>(a);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-    int ql, kl;
-    lens(a, pl.b, ql, kl);
+    const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
     const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
-    const int g = r / a.Sq, pos = r - g * a.Sq;
-    const bool row_ok = r < a.R && pos < ql;
+    const Row me = row_of(a, ql, r);
+    const int g = me.g, pos = me.pos;
+    const bool row_ok = me.ok;
     const int off = kl - ql;
-    int lo, hi, kend = kl;
-    span(a, r0, min(r0 + NW * 32, a.R), lo, hi);
-    if (a.causal) kend = min(kl, min(hi, ql - 1) + off + 1);
-    if (lo >= ql) kend = 0;
+    int lo = 0, kend = 0;
+    if (r0 < rv) {
+        int hi;
+        span(ql, r0, min(r0 + NW * 32, rv), lo, hi);
+        kend = a.causal ? min(kl, hi + off + 1) : kl;
+    }
     int t0 = 0, t1 = (max(kend, 0) + KT - 1) / KT;
-    if (a.nsplit > 1) {
-        t0 = pl.split * a.split_tiles;
-        t1 = min(t1, t0 + a.split_tiles);
+    if (a.nsplit > 1) {                           // the pieces follow the keys that there are
+        const int per = (t1 + a.nsplit - 1) / a.nsplit;
+        t0 = pl.split * per;
+        t1 = min(t1, t0 + per);
     }
     const long es = sizeof(T);
     const char* kb = a.k + (pl.b * a.k_sb + pl.kh * a.k_sh) * es;
@@ -369,7 +436,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
     }
     l += other_half(l);
     if (r >= a.R) return;
-    const long hrow = ((long)pl.b * a.Hkv + pl.kh) * a.R + r;       // = ((b * H + head) * Sq + pos)
+    const long hrow = ((long)pl.b * a.H + pl.kh * a.G + g) * a.Sq + pos;
     if (a.nsplit > 1) {
         const long prow = (long)pl.split * a.B * a.Hkv * a.R + hrow;
         float* po = a.part + prow * D;
@@ -482,25 +549,28 @@ __device__ __forceinline__ bool join_sum(const Args& a, const float* part, long 
 // ------------------------------------------------------------------------------------------------ backward, query side
 // The forward's shape; delta_i from the saved o, kept for the key side.
 template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64, 2) void dq_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = KT * pitch<T, D>();
-    const Place pl = place(a, a.causal);
+    const Place pl = place<NW * 32, false>(a);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-    int ql, kl;
-    lens(a, pl.b, ql, kl);
+    const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
     const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
-    const int g = r / a.Sq, pos = r - g * a.Sq;
-    const bool row_ok = r < a.R && pos < ql;
+    const Row me = row_of(a, ql, r);
+    const int g = me.g, pos = me.pos;
+    const bool row_ok = me.ok;
     const int off = kl - ql;
-    int lo, hi, kend = kl;
-    span(a, r0, min(r0 + NW * 32, a.R), lo, hi);
-    if (a.causal) kend = min(kl, min(hi, ql - 1) + off + 1);
-    if (lo >= ql) kend = 0;
+    int lo = 0, kend = 0;
+    if (r0 < rv) {
+        int hi;
+        span(ql, r0, min(r0 + NW * 32, rv), lo, hi);
+        kend = a.causal ? min(kl, hi + off + 1) : kl;
+    }
     int t0 = 0, t1 = (max(kend, 0) + KT - 1) / KT;
-    if (a.nsplit > 1) {
-        t0 = pl.split * a.split_tiles;
-        t1 = min(t1, t0 + a.split_tiles);
+    if (a.nsplit > 1) {                           // the pieces follow the keys that there are
+        const int per = (t1 + a.nsplit - 1) / a.nsplit;
+        t0 = pl.split * per;
+        t1 = min(t1, t0 + per);
     }
     const long es = sizeof(T);
     const int head = pl.kh * a.G + g;
@@ -509,7 +579,7 @@ __global__ __launch_bounds__(NW * 64, 2) void dq_kernel(Args a) {
     const char* grow = a.doo + (pl.b * a.g_sb + pos * a.g_ss + head * a.g_sh) * es;
     const Frag<T, D> qf = load_frag<T, D>(a.q + (pl.b * a.q_sb + pos * a.q_ss + head * a.q_sh) * es, row_ok);
     const Frag<T, D> gf = load_frag<T, D>(grow, row_ok);
-    const long hrow = ((long)pl.b * a.Hkv + pl.kh) * a.R + r;
+    const long hrow = ((long)pl.b * a.H + head) * a.Sq + pos;
     const long orow = (((long)pl.b * a.Sq + pos) * a.H + head) * D * es;
     float dl, lse = INFINITY;
     {
@@ -603,11 +673,9 @@ template <typename T, int D, int NW, int RT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = RT * pitch<T, D>(), BUF = 2 * TB + RT * 8;
-    const Place pl = place(a, false);
+    const Place pl = place<NW * 32, true>(a);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-    int ql, kl;
-    lens(a, pl.b, ql, kl);
-    const int off = kl - ql;
+    const int ql = pl.ql, kl = pl.kl, off = kl - ql, rv = a.G * ql;
     const int key0 = pl.tile * NW * 32, key = key0 + w * 32 + (lane & 31);
     const bool key_ok = key < kl;
     const long es = sizeof(T);
@@ -615,23 +683,25 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
     const Frag<T, D> vf = load_frag<T, D>(a.v + (pl.b * a.v_sb + key * a.v_ss + pl.kh * a.v_sh) * es, key_ok);
     const char* qb = a.q + (pl.b * a.q_sb + (long)pl.kh * a.G * a.q_sh) * es;
     const char* gb = a.doo + (pl.b * a.g_sb + (long)pl.kh * a.G * a.g_sh) * es;
-    const long hrow0 = ((long)pl.b * a.Hkv + pl.kh) * a.R;
+    const long hrow0 = ((long)pl.b * a.H + pl.kh * a.G) * a.Sq;
     f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = zero16();
 
-    int t1 = (a.R + RT - 1) / RT, t = 0;
-    if (a.nsplit > 1) {
-        t = pl.split * a.split_tiles;
-        t1 = min(t1, t + a.split_tiles);
+    int t1 = (rv + RT - 1) / RT, t = 0;
+    if (a.nsplit > 1) {                           // the pieces follow the rows that there are
+        const int per = (t1 + a.nsplit - 1) / a.nsplit;
+        t = pl.split * per;
+        t1 = min(t1, t + per);
     }
     if (key0 >= kl) t = t1;
     // the next tile of rows with a valid pair, from t on
     auto next = [&](int t) {
         for (; t < t1; ++t) {
             int lo, hi;
-            span(a, t * RT, min(t * RT + RT, a.R), lo, hi);
-            if (lo < ql && (!a.causal || min(hi, ql - 1) + off >= key0)) break;
+            if (!a.causal) break;
+            span(ql, t * RT, min(t * RT + RT, rv), lo, hi);
+            if (hi + off >= key0) break;
         }
         return t;
     };
@@ -639,13 +709,18 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
     Stage<T, D, RT, NW * 64> qs, gs;
     float st_lse = 0.f, st_dl = 0.f;
     auto request = [&](int t) {
-        qs.load_rows(qb, a.q_ss * es, a.q_sh * es, t * RT, a.R, a.Sq, ql);
-        gs.load_rows(gb, a.g_ss * es, a.g_sh * es, t * RT, a.R, a.Sq, ql);
+        qs.load_rows(qb, a.q_ss * es, a.q_sh * es, t * RT, rv, ql);
+        gs.load_rows(gb, a.g_ss * es, a.g_sh * es, t * RT, rv, ql);
         if (threadIdx.x < RT) {
             const int r = t * RT + threadIdx.x;
-            const bool ok = r < a.R && r - r / a.Sq * a.Sq < ql;
-            st_lse = ok ? a.lse[hrow0 + r] - p_shift<T>() : INFINITY;
-            st_dl = ok ? a.delta[hrow0 + r] * unshift : 0.f;
+            st_lse = INFINITY;
+            st_dl = 0.f;
+            if (r < rv) {
+                const int g = r / ql;
+                const long at = hrow0 + (long)g * a.Sq + (r - g * ql);
+                st_lse = a.lse[at] - p_shift<T>();
+                st_dl = a.delta[at] * unshift;
+            }
         }
     };
     auto put = [&](char* buf) {
@@ -667,9 +742,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
         const char* buf = smem + cur * BUF;
         const int tn = next(t + 1);
         if (tn < t1) request(tn);
-        int lo, hi;
-        span(a, t * RT, min(t * RT + RT, a.R), lo, hi);
-        const bool edge = a.causal && lo + off < key0 + NW * 32 - 1;
+        bool edge = false;
+        if (a.causal) {
+            int lo, hi;
+            span(ql, t * RT, min(t * RT + RT, rv), lo, hi);
+            edge = lo + off < key0 + NW * 32 - 1;
+        }
 #pragma unroll
         for (int u = 0; u < RT / 32; ++u) {
             f32x16 s = mul_rows<T, D>(buf, u * 32, kf, zero16());
@@ -684,7 +762,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = t * RT + u * 32 + acc_row(i, h), p = r - r / a.Sq * a.Sq;
+                    const int r = t * RT + u * 32 + acc_row(i, h), p = r - r / ql * ql;
                     if (p + off < key) s[i] = 0.f;
                 }
             }
@@ -717,6 +795,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
                 y[j] = key_ok ? dv[d][4 * q4 + j] * unshift : 0.f;
             }
             if (a.nsplit > 1) {
+                if (!key_ok) continue;            // the joining kernel knows
                 *reinterpret_cast<f32x4*>(a.part + part0 * D + ch) = x;
                 *reinterpret_cast<f32x4*>(a.part + (total + part0) * D + ch) = y;
             } else {
@@ -726,13 +805,19 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
         }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void dkv_join_kernel(Args a, long n4) {
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
+    const long n4 = (long)a.B * a.Sk * a.Hkv * (D / 4);
     const int per = 256 / a.sg, sg = (int)threadIdx.x / per;
     const long e = (long)blockIdx.x * per + threadIdx.x - sg * per;
+    const long row = e / ((D / 4) * a.Hkv);                        // b * Sk + key
+    const int b = (int)(row / a.Sk);
+    int ql = 0, kl = 0;
+    if (e < n4) lens(a, b, ql, kl);
+    const bool there = e < n4 && (int)(row - (long)b * a.Sk) < kl;
     f32x4 x, y;
-    const bool mine = join_sum(a, a.part, n4, e, sg, x);
-    join_sum(a, a.part + (size_t)a.nsplit * n4 * 4, n4, e, sg, y);
+    const bool mine = join_sum(a, a.part, n4, there ? e : n4, sg, x);
+    join_sum(a, a.part + (size_t)a.nsplit * n4 * 4, n4, there ? e : n4, sg, y);
     if (!mine || e >= n4) return;
     store4<T>(a.dk + e * 4 * sizeof(T), x[0], x[1], x[2], x[3]);
     store4<T>(a.dv + e * 4 * sizeof(T), y[0], y[1], y[2], y[3]);
@@ -740,30 +825,32 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(Args a, long n4) {
 
 // ------------------------------------------------------------------------------------------------ launches
 struct Plan {
-    int nw, tile, ntiles, nsplit, split_tiles;      // waves per workgroup, contraction rows per tile, tiles of own rows
+    int nw, tile, ntiles, nsplit, occ;              // waves per workgroup, contraction rows per tile, tiles of own rows
     size_t lds;
 };
 
-// `rows` own rows in tiles of 32 per wave, `len` rows to walk.  Four waves share what they walk; where that leaves most
-// of the card idle, one wave per workgroup and the walk cut into pieces that a second launch joins.
-static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats) {
+// `rows` own rows in tiles of 32 per wave, `len` rows to walk; `occ` workgroups of four waves fit on a compute unit.  Four
+// waves share what they walk; where that leaves most of the card idle, one wave per workgroup.  The walk is cut into pieces,
+// which a second launch joins, until there is work for every wave slot — twice that for the causal order, whose workgroups
+// are of very different length, and half again as much where lengths will leave some without work.
+static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats, int occ, bool causal, bool ragged) {
     Plan p;
-    const long wg4 = nbh * ((rows + 127) / 128);
-    p.nw = wg4 >= 256 ? 4 : 1;
+    p.occ = occ;
+    const long wg4 = nbh * ((rows + 127) / 128), cus = compute_units();
+    p.nw = wg4 >= cus ? 4 : 1;
     p.tile = p.nw == 4 && esize * D <= 256 ? 64 : 32;
     p.ntiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
     p.nsplit = 1;
     const int tiles = (len + p.tile - 1) / p.tile;
-    const long wg = nbh * p.ntiles, want = p.nw == 4 ? 256 : 1024;
-    if (wg > 0 && wg < want && tiles > 1) {
+    const long wg = nbh * p.ntiles;
+    long want = p.nw == 4 ? cus * occ : 4 * cus;
+    if (p.nw == 4) want = causal ? 2 * want : ragged ? want + want / 2 : want;
+    const int least = p.nw == 4 ? 4 : 2;          // tiles per piece
+    if (wg > 0 && wg < want && tiles >= 2 * least) {
         long ns = (want + wg - 1) / wg;
-        if (ns > tiles / 2) ns = tiles / 2;           // at least two tiles per piece
-        if (ns > 64) ns = 64;
-        if (ns > 1) p.nsplit = (int)ns;
+        if (ns > tiles / least) ns = tiles / least;
+        p.nsplit = (int)(ns > 64 ? 64 : ns);
     }
-    p.split_tiles = (tiles + p.nsplit - 1) / p.nsplit;
-    if (p.split_tiles < 1) p.split_tiles = 1;
-    p.nsplit = tiles > 0 ? (tiles + p.split_tiles - 1) / p.split_tiles : 1;
     p.lds = 2 * ((size_t)2 * p.tile * (D * esize + 16) + (stats ? p.tile * 8 : 0));
     return p;
 }
@@ -779,9 +866,10 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const int es = (int)esize_of(d.dtype), G = d.H / d.Hkv;
     const long nbh = (long)d.B * d.Hkv;
     const int R = G * d.Sq;
-    z.f = make_plan(es, d.D, nbh, R, d.Sk, false);
-    z.q = z.f;
-    z.k = make_plan(es, d.D, nbh, d.Sk, R, true);
+    const bool causal = d.causal != 0, ragged = d.q_len || d.k_len;
+    z.f = make_plan(es, d.D, nbh, R, d.Sk, false, 2, causal, ragged);
+    z.q = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
+    z.k = make_plan(es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged);
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
     z.fwd = z.f.nsplit > 1 ? z.f.nsplit * rows * (d.D + 2) * 4 : 0;
     const size_t bq = z.q.nsplit > 1 ? z.q.nsplit * rows * d.D * 4 : 0;
@@ -804,7 +892,7 @@ static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a,
 static void use(Args& a, const Plan& p) {
     a.ntiles = p.ntiles;
     a.nsplit = p.nsplit;
-    a.split_tiles = p.split_tiles;
+    a.fold = p.occ >= 2 ? compute_units() : 1 << 29;
 }
 
 // groups that share out the splits of one value in a joining kernel of n4 x 4 values: until the launch fills the card
@@ -851,8 +939,7 @@ static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
     if (e || a.nsplit == 1) return e;
     const long n4 = keys * D / 4;
     a.sg = join_groups(a.nsplit, n4, 16);
-    hipLaunchKernelGGL(dkv_join_kernel<T>, dim3((unsigned)((n4 * a.sg + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a, n4);
-    return check_launch("set_attention dkv_join_kernel");
+    return launch(dkv_join_kernel<T, D>, (n4 * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dkv_join_kernel");
 }
 
 static bool aligned(const void* p, const int64_t* s, int dtype, int extra) {
@@ -872,7 +959,7 @@ static int check_desc(const char* who, const cmvae_set_attn* d) {
     CMVAE_REQUIRE(d->scale >= 1e-30f && d->scale <= 1e30f, "%s: scale %g (a positive finite number)", who, (double)d->scale);
     const Sizes z = sizes_of(*d);
     const long nbh = (long)d->B * d->Hkv;
-    CMVAE_REQUIRE(nbh * z.f.ntiles * z.f.nsplit < (1L << 31) && nbh * z.k.ntiles * z.k.nsplit < (1L << 31) &&
+    CMVAE_REQUIRE(nbh * z.f.ntiles * z.f.nsplit < (1L << 31) && nbh * z.q.ntiles * z.q.nsplit < (1L << 31) && nbh * z.k.ntiles * z.k.nsplit < (1L << 31) &&
                       nbh * (d->H / d->Hkv) * d->Sq * (d->D / 4) / 256 < (1L << 31) - 1 &&
                       nbh * d->Sk * (d->D / 4) / 256 < (1L << 31) - 1,
                   "%s: the problem needs more than 2^31 workgroups", who);
