@@ -15,8 +15,11 @@
 // second factor of the next product (o^T = V^T P^T, dq^T = K^T dS^T).  The dkv kernel holds 32 keys per wave and forms
 // S (queries x keys) for dv^T = dO^T P and dk^T = Q^T dS.  No probability is ever stored.
 //
-// Element types: fp32 on v_mfma_f32_32x32x2_f32, bf16 / fp16 on the 32x32x16 forms.  Scores, softmax statistics,
-// delta and every accumulator are fp32; in the 16-bit types P and dS are rounded once (to nearest) to be factors.
+// Element types: bf16 and fp16 on their 32x32x16 instructions; fp32 on the bf16 one, each value as the exact sum of three
+// bf16 pieces (to nearest, 8 + 8 + 8 bits) and each product as the six piece products that reach above 2^-24 of it —
+// fp32's own accuracy (test_gpu_set_attention.py holds it to fp32 tolerances) at 6/16 of the fp32 instruction's cycles.  An
+// infinite fp32 input makes NaN of its rows.  Scores, softmax statistics, delta and every accumulator are fp32; in the
+// 16-bit types P and dS are rounded once (to nearest) to be factors.
 #include "common.h"
 
 #include <cmath>
@@ -54,11 +57,46 @@ struct Vec8 {};
 template <> struct Vec8<__bf16> { typedef bf16x8 type; };
 template <> struct Vec8<_Float16> { typedef f16x8 type; };
 
+// What the matrix instructions take for a T: itself, or three bf16 planes for fp32.
+template <typename T> struct Elem { typedef T type; static constexpr int P = 1; };
+template <> struct Elem<float> { typedef __bf16 type; static constexpr int P = 3; };
+
 // Second factor of a product over D channels, 32 columns: D / 2 values per lane.
 template <typename T, int D>
 struct Frag {
-    u32x4 x[D * sizeof(T) / 32];
+    u32x4 x[Elem<T>::P][D / 16];
 };
+
+// x - (one half of a packed bf16 pair) in one v_dot2c_f32_bf16 with (-1, 0) / (0, -1); the selectors are made once per kernel
+// and kept in registers (as an inline constant the assembler's -1.0 is not the packed pattern).
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+struct Sel {
+    bf16x2 lo, hi;
+};
+__device__ __forceinline__ Sel make_sel() {
+    unsigned a = 0x0000bf80u, b = 0xbf800000u;
+    asm volatile("" : "+v"(a), "+v"(b));
+    return Sel{__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b)};
+}
+__device__ __forceinline__ void split2(float x, float y, const Sel& q, unsigned (&p)[3]) {
+    const bf16x2 a = __builtin_convertvector(f32x2{x, y}, bf16x2);
+    const float rx = __builtin_amdgcn_fdot2_f32_bf16(a, q.lo, x, false), ry = __builtin_amdgcn_fdot2_f32_bf16(a, q.hi, y, false);
+    const bf16x2 b = __builtin_convertvector(f32x2{rx, ry}, bf16x2);
+    const float sx = __builtin_amdgcn_fdot2_f32_bf16(b, q.lo, rx, false), sy = __builtin_amdgcn_fdot2_f32_bf16(b, q.hi, ry, false);
+    p[0] = __builtin_bit_cast(unsigned, a);
+    p[1] = __builtin_bit_cast(unsigned, b);
+    p[2] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{sx, sy}, bf16x2));
+}
+__device__ __forceinline__ void split8(const float (&v)[8], const Sel& q, u32x4 (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        unsigned t[3];
+        split2(v[2 * i], v[2 * i + 1], q, t);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) p[j][i] = t[j];
+    }
+}
 
 template <typename T>
 __device__ __forceinline__ f32x16 mma16(u32x4 a, u32x4 b, f32x16 c) {
@@ -66,6 +104,20 @@ __device__ __forceinline__ f32x16 mma16(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// a product of P planes each, small terms first
+template <typename T>
+__device__ __forceinline__ f32x16 mma(const u32x4 (&a)[Elem<T>::P], const u32x4 (&b)[Elem<T>::P], f32x16 c) {
+    typedef typename Elem<T>::type E;
+    if constexpr (Elem<T>::P == 3) {
+        c = mma16<E>(a[2], b[0], c);
+        c = mma16<E>(a[0], b[2], c);
+        c = mma16<E>(a[1], b[1], c);
+        c = mma16<E>(a[1], b[0], c);
+        c = mma16<E>(a[0], b[1], c);
+    }
+    return mma16<E>(a[0], b[0], c);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -85,98 +137,122 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32);
 __device__ __forceinline__ constexpr int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
 // The LDS pitch of a tile row: 16 bytes more than the row, so that the 32 rows of a fragment read start in different banks.
-template <typename T, int D> __host__ __device__ constexpr int pitch() { return D * (int)sizeof(T) + 16; }
+template <int D> __host__ __device__ constexpr int pitch() { return D * 2 + 16; }
 
-// ---- first factor = 32 rows of an LDS tile, contraction over the D channels -------------------------------------------
-// The contraction's order is free as long as both factors agree: lane half h takes channels 8c + 4h .. + 3 of fp32
-// (16c + 8h .. + 7 of 16-bit) rows, one 16-byte read.
-template <typename T, int D>
+// ---- first factor = 32 rows of an LDS tile of ROWS rows (P planes), contraction over the D channels ------------------
+// The contraction's order is free as long as both factors agree: lane half h takes channels 16c + 8h .. + 7, one 16-byte
+// read per plane.
+template <typename T, int D, int ROWS>
 __device__ __forceinline__ f32x16 mul_rows(const char* tile, int row0, const Frag<T, D>& b, f32x16 acc) {
+    constexpr int P = Elem<T>::P;
     const int lane = threadIdx.x & 63;
-    const char* p = tile + (row0 + (lane & 31)) * pitch<T, D>() + (lane >> 5) * 16;
-    constexpr int NC = D * sizeof(T) / 32;
+    const char* p = tile + (row0 + (lane & 31)) * pitch<D>() + (lane >> 5) * 16;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(p + c * 32);
-        if constexpr (std::is_same<T, float>::value) {
-            const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b.x[c]);
+    for (int c = 0; c < D / 16; ++c) {
+        u32x4 a[P], y[P];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], acc, 0, 0, 0);
-        } else {
-            acc = mma16<T>(a, b.x[c], acc);
+        for (int i = 0; i < P; ++i) {
+            a[i] = *reinterpret_cast<const u32x4*>(p + i * ROWS * pitch<D>() + c * 32);
+            y[i] = b.x[i][c];
         }
+        acc = mma<T>(a, y, acc);
     }
     return acc;
 }
 
 // ---- first factor = 32 channels x 32 rows of an LDS tile (transposed), second factor = a 32 x 32 accumulator --------
-// Register r of the accumulator is tile row acc_row(r, h), which fixes the contraction's order.  fp32: one value per
-// lane and instruction.  16-bit: registers 8s .. 8s + 7 are one instruction's eight; the matching first factor — four
-// rows at one channel, twice — comes from the transposing LDS read (16 lanes name 4 rows x 16 channels, lane i
-// receives channel i of the four rows).
-template <typename T, int D>
-__device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, f32x16 (&acc)[D / 32]) {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+// Register r of the accumulator is tile row acc_row(r, h), which fixes the contraction's order: registers 8s .. 8s + 7 are
+// one instruction's eight; the matching first factor — four rows at one channel, twice — comes from the transposing LDS
+// read (16 lanes name 4 rows x 16 channels, lane i receives channel i of the four rows).
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, const Sel& sel, f32x16 (&acc)[D / 32]) {
+    constexpr int P = Elem<T>::P;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const int lane = threadIdx.x & 63, h = lane >> 5, i = lane & 15;
+    const char* p = tile + (row0 + 4 * h + (i >> 2)) * pitch<D>() + (lane & 16) * 2 + (i & 3) * 8;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        u32x4 b[P];
+        if constexpr (P == 3) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = w[8 * s + j];
+            split8(v, sel, b);
+        } else {
+            typename Vec8<T>::type v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (T)w[8 * s + j];
+            b[0] = __builtin_bit_cast(u32x4, v);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+            u32x4 a[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const char* at = p + (k * ROWS + 16 * s) * pitch<D>() + d * 64;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 8 * pitch<D>()));
+                a[k] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+            acc[d] = mma<T>(a, b, acc[d]);
+        }
+    }
+}
+
+// eight channels of a row as fp32
+template <typename T>
+__device__ __forceinline__ void load8(const char* p, float (&v)[8]) {
     if constexpr (std::is_same<T, float>::value) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 16);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const char* p = tile + (row0 + acc_row(r, h)) * pitch<T, D>() + (lane & 31) * 4;
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(p + d * 128), w[r], acc[d], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) {
+            v[j] = a[j];
+            v[4 + j] = b[j];
         }
     } else {
-        typedef typename Vec8<T>::type V8;
-        const int i = lane & 15;
-        const char* p = tile + (row0 + 4 * h + (i >> 2)) * pitch<T, D>() + (lane & 16) * 2 + (i & 3) * 8;
+        const typename Vec8<T>::type a = *reinterpret_cast<const typename Vec8<T>::type*>(p);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            V8 b;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = (T)w[8 * s + j];
-            const u32x4 bu = __builtin_bit_cast(u32x4, b);
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const char* a = p + 16 * s * pitch<T, D>() + d * 64;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(a + 8 * pitch<T, D>()));
-                const s16x8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[d] = mma16<T>(__builtin_bit_cast(u32x4, av), bu, acc[d]);
-            }
-        }
+        for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
     }
 }
 
 // one row as a second factor (lane & 31 = column); rows that are not there are zero
 template <typename T, int D>
-__device__ __forceinline__ Frag<T, D> load_frag(const char* row, bool there) {
+__device__ __forceinline__ Frag<T, D> load_frag(const char* row, bool there, const Sel& sel) {
     const int h = (threadIdx.x & 63) >> 5;
     Frag<T, D> f;
 #pragma unroll
-    for (int c = 0; c < (int)(D * sizeof(T) / 32); ++c) {
-        f.x[c] = u32x4{0, 0, 0, 0};
-        if (there) f.x[c] = *reinterpret_cast<const u32x4*>(row + c * 32 + h * 16);
+    for (int c = 0; c < D / 16; ++c) {
+        const char* p = row + (16 * c + 8 * h) * sizeof(T);
+        if constexpr (Elem<T>::P == 3) {
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (there) load8<T>(p, v);
+            u32x4 x[3];
+            split8(v, sel, x);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) f.x[i][c] = x[i];
+        } else {
+            f.x[0][c] = u32x4{0, 0, 0, 0};
+            if (there) f.x[0][c] = *reinterpret_cast<const u32x4*>(p);
+        }
     }
     return f;
 }
 
+// the product of two rows, each lane half over its half of the channels
 template <typename T, int D>
-__device__ __forceinline__ float dot_frag(const Frag<T, D>& a, const Frag<T, D>& b) {
+__device__ __forceinline__ float dot_rows(const char* x, const char* y, bool there) {
+    const int h = (threadIdx.x & 63) >> 5;
     float s = 0.f;
+    if (there)
 #pragma unroll
-    for (int c = 0; c < (int)(D * sizeof(T) / 32); ++c) {
-        if constexpr (std::is_same<T, float>::value) {
-            const f32x4 x = __builtin_bit_cast(f32x4, a.x[c]), y = __builtin_bit_cast(f32x4, b.x[c]);
+        for (int c = 0; c < D / 16; ++c) {
+            float a[8], b[8];
+            load8<T>(x + (16 * c + 8 * h) * sizeof(T), a);
+            load8<T>(y + (16 * c + 8 * h) * sizeof(T), b);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s = fmaf(x[j], y[j], s);
-        } else {
-            typedef typename Vec8<T>::type V8;
-            const V8 x = __builtin_bit_cast(V8, a.x[c]), y = __builtin_bit_cast(V8, b.x[c]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
+            for (int j = 0; j < 8; ++j) s = fmaf(a[j], b[j], s);
         }
-    }
     return s + other_half(s);
 }
 
@@ -230,11 +306,21 @@ struct Stage {
             }
         }
     }
-    __device__ __forceinline__ void put(char* tile) const {
+    __device__ __forceinline__ void put(char* tile, const Sel& sel) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int id = i * THREADS + threadIdx.x;
-            *reinterpret_cast<u32x4*>(tile + (id / CPR) * pitch<T, D>() + (id % CPR) * 16) = x[i];
+            char* at = tile + (id / CPR) * pitch<D>() + (id % CPR) * (Elem<T>::P == 3 ? 8 : 16);
+            if constexpr (Elem<T>::P == 3) {
+                const f32x4 v = __builtin_bit_cast(f32x4, x[i]);
+                unsigned a[3], b[3];
+                split2(v[0], v[1], sel, a);
+                split2(v[2], v[3], sel, b);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(at + k * ROWS * pitch<D>()) = make_uint2(a[k], b[k]);
+            } else {
+                *reinterpret_cast<u32x4*>(at) = x[i];
+            }
         }
     }
 };
@@ -344,10 +430,11 @@ __device__ __forceinline__ void span(int ql, int r0, int r1, int& lo, int& hi) {
 // NW waves of 32 rows; keys in tiles of KT through LDS, two buffers.  Running maximum m (log2 units) and sum l per row.
 // nsplit > 1: a workgroup covers split_tiles tiles and leaves (acc, m, l) for the joining kernel.
 template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int TB = KT * pitch<T, D>();
+    constexpr int TB = Elem<T>::P * KT * pitch<D>();
     const Place pl = place<NW * 32, false>(a);
+    const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
     const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
@@ -371,7 +458,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
     const char* kb = a.k + (pl.b * a.k_sb + pl.kh * a.k_sh) * es;
     const char* vb = a.v + (pl.b * a.v_sb + pl.kh * a.v_sh) * es;
     const char* qrow = a.q + (pl.b * a.q_sb + pos * a.q_ss + (pl.kh * a.G + g) * a.q_sh) * es;
-    const Frag<T, D> qf = load_frag<T, D>(qrow, row_ok);
+    const Frag<T, D> qf = load_frag<T, D>(qrow, row_ok, sel);
     f32x16 acc[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) acc[d] = zero16();
@@ -382,8 +469,8 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
     if (t0 < t1) {
         ks.load(kb, a.k_ss * es, t0 * KT, kl);
         vs.load(vb, a.v_ss * es, t0 * KT, kl);
-        ks.put(smem);
-        vs.put(smem + TB);
+        ks.put(smem, sel);
+        vs.put(smem + TB, sel);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -395,7 +482,7 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
         }
         f32x16 s[KT / 32];
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) s[u] = mul_rows<T, D>(kt, u * 32, qf, zero16());
+        for (int u = 0; u < KT / 32; ++u) s[u] = mul_rows<T, D, KT>(kt, u * 32, qf, zero16());
         const int k0 = t * KT;
         if (k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1)) {
 #pragma unroll
@@ -426,11 +513,11 @@ __global__ __launch_bounds__(NW * 64, 2) void fwd_kernel(Args a) {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= al;
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) mul_cols<T, D>(vt, u * 32, s[u], acc);
+        for (int u = 0; u < KT / 32; ++u) mul_cols<T, D, KT>(vt, u * 32, s[u], sel, acc);
         if (t + 1 < t1) {
             char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
-            ks.put(nx);
-            vs.put(nx + TB);
+            ks.put(nx, sel);
+            vs.put(nx + TB, sel);
         }
         __syncthreads();
     }
@@ -551,8 +638,9 @@ __device__ __forceinline__ bool join_sum(const Args& a, const float* part, long 
 template <typename T, int D, int NW, int KT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int TB = KT * pitch<T, D>();
+    constexpr int TB = Elem<T>::P * KT * pitch<D>();
     const Place pl = place<NW * 32, false>(a);
+    const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
     const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
@@ -577,14 +665,13 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
     const char* kb = a.k + (pl.b * a.k_sb + pl.kh * a.k_sh) * es;
     const char* vb = a.v + (pl.b * a.v_sb + pl.kh * a.v_sh) * es;
     const char* grow = a.doo + (pl.b * a.g_sb + pos * a.g_ss + head * a.g_sh) * es;
-    const Frag<T, D> qf = load_frag<T, D>(a.q + (pl.b * a.q_sb + pos * a.q_ss + head * a.q_sh) * es, row_ok);
-    const Frag<T, D> gf = load_frag<T, D>(grow, row_ok);
+    const Frag<T, D> qf = load_frag<T, D>(a.q + (pl.b * a.q_sb + pos * a.q_ss + head * a.q_sh) * es, row_ok, sel);
+    const Frag<T, D> gf = load_frag<T, D>(grow, row_ok, sel);
     const long hrow = ((long)pl.b * a.H + head) * a.Sq + pos;
     const long orow = (((long)pl.b * a.Sq + pos) * a.H + head) * D * es;
     float dl, lse = INFINITY;
     {
-        const Frag<T, D> of = load_frag<T, D>(a.att + orow, row_ok);
-        dl = dot_frag<T, D>(gf, of);
+        dl = dot_rows<T, D>(grow, a.att + orow, row_ok);
         if (row_ok) lse = a.lse[hrow];
         if (h == 0 && r < a.R && pl.split == 0) a.delta[hrow] = dl;
     }
@@ -597,8 +684,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
     if (t0 < t1) {
         ks.load(kb, a.k_ss * es, t0 * KT, kl);
         vs.load(vb, a.v_ss * es, t0 * KT, kl);
-        ks.put(smem);
-        vs.put(smem + TB);
+        ks.put(smem, sel);
+        vs.put(smem + TB, sel);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -612,8 +699,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
         const bool edge = k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1);
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
-            f32x16 s = mul_rows<T, D>(kt, u * 32, qf, zero16());
-            f32x16 dp = mul_rows<T, D>(vt, u * 32, gf, zero16());
+            f32x16 s = mul_rows<T, D, KT>(kt, u * 32, qf, zero16());
+            f32x16 dp = mul_rows<T, D, KT>(vt, u * 32, gf, zero16());
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = exp2_raw(fmaf(s[i], a.c, -lse)) * (dp[i] - dl);
             if (edge) {
@@ -621,12 +708,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
                 for (int i = 0; i < 16; ++i)
                     if (k0 + u * 32 + acc_row(i, h) >= klast) s[i] = 0.f;
             }
-            mul_cols<T, D>(kt, u * 32, s, acc);
+            mul_cols<T, D, KT>(kt, u * 32, s, sel, acc);
         }
         if (t + 1 < t1) {
             char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
-            ks.put(nx);
-            vs.put(nx + TB);
+            ks.put(nx, sel);
+            vs.put(nx + TB, sel);
         }
         __syncthreads();
     }
@@ -672,15 +759,16 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 template <typename T, int D, int NW, int RT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int TB = RT * pitch<T, D>(), BUF = 2 * TB + RT * 8;
+    constexpr int TB = Elem<T>::P * RT * pitch<D>(), BUF = 2 * TB + RT * 8;
     const Place pl = place<NW * 32, true>(a);
+    const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, off = kl - ql, rv = a.G * ql;
     const int key0 = pl.tile * NW * 32, key = key0 + w * 32 + (lane & 31);
     const bool key_ok = key < kl;
     const long es = sizeof(T);
-    const Frag<T, D> kf = load_frag<T, D>(a.k + (pl.b * a.k_sb + key * a.k_ss + pl.kh * a.k_sh) * es, key_ok);
-    const Frag<T, D> vf = load_frag<T, D>(a.v + (pl.b * a.v_sb + key * a.v_ss + pl.kh * a.v_sh) * es, key_ok);
+    const Frag<T, D> kf = load_frag<T, D>(a.k + (pl.b * a.k_sb + key * a.k_ss + pl.kh * a.k_sh) * es, key_ok, sel);
+    const Frag<T, D> vf = load_frag<T, D>(a.v + (pl.b * a.v_sb + key * a.v_ss + pl.kh * a.v_sh) * es, key_ok, sel);
     const char* qb = a.q + (pl.b * a.q_sb + (long)pl.kh * a.G * a.q_sh) * es;
     const char* gb = a.doo + (pl.b * a.g_sb + (long)pl.kh * a.G * a.g_sh) * es;
     const long hrow0 = ((long)pl.b * a.H + pl.kh * a.G) * a.Sq;
@@ -724,8 +812,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
         }
     };
     auto put = [&](char* buf) {
-        qs.put(buf);
-        gs.put(buf + TB);
+        qs.put(buf, sel);
+        gs.put(buf + TB, sel);
         if (threadIdx.x < RT) {
             reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
             reinterpret_cast<float*>(buf + 2 * TB)[RT + threadIdx.x] = st_dl;
@@ -750,8 +838,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
         }
 #pragma unroll
         for (int u = 0; u < RT / 32; ++u) {
-            f32x16 s = mul_rows<T, D>(buf, u * 32, kf, zero16());
-            f32x16 dp = mul_rows<T, D>(buf + TB, u * 32, vf, zero16());
+            f32x16 s = mul_rows<T, D, RT>(buf, u * 32, kf, zero16());
+            f32x16 dp = mul_rows<T, D, RT>(buf + TB, u * 32, vf, zero16());
             const float* st = reinterpret_cast<const float*>(buf + 2 * TB) + u * 32 + 4 * h;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
@@ -766,14 +854,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_ker
                     if (p + off < key) s[i] = 0.f;
                 }
             }
-            mul_cols<T, D>(buf + TB, u * 32, s, dv);
+            mul_cols<T, D, RT>(buf + TB, u * 32, s, sel, dv);
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 const f32x4 dl = *reinterpret_cast<const f32x4*>(st + RT + 8 * q4);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[4 * q4 + j] *= fmaf(dp[4 * q4 + j], unshift, -dl[j]);
             }
-            mul_cols<T, D>(buf, u * 32, s, dk);
+            mul_cols<T, D, RT>(buf, u * 32, s, sel, dk);
         }
         if (tn < t1) put(smem + (cur ^ 1) * BUF);
         __syncthreads();
@@ -838,7 +926,7 @@ static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats,
     p.occ = occ;
     const long wg4 = nbh * ((rows + 127) / 128), cus = compute_units();
     p.nw = wg4 >= cus ? 4 : 1;
-    p.tile = p.nw == 4 && esize * D <= 256 ? 64 : 32;
+    p.tile = p.nw == 4 && esize == 2 ? 64 : 32;
     p.ntiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
     p.nsplit = 1;
     const int tiles = (len + p.tile - 1) / p.tile;
@@ -851,7 +939,7 @@ static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats,
         if (ns > tiles / least) ns = tiles / least;
         p.nsplit = (int)(ns > 64 ? 64 : ns);
     }
-    p.lds = 2 * ((size_t)2 * p.tile * (D * esize + 16) + (stats ? p.tile * 8 : 0));
+    p.lds = 2 * ((size_t)2 * (esize == 4 ? 3 : 1) * p.tile * (D * 2 + 16) + (stats ? p.tile * 8 : 0));
     return p;
 }
 
@@ -867,7 +955,7 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const long nbh = (long)d.B * d.Hkv;
     const int R = G * d.Sq;
     const bool causal = d.causal != 0, ragged = d.q_len || d.k_len;
-    z.f = make_plan(es, d.D, nbh, R, d.Sk, false, 2, causal, ragged);
+    z.f = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
     z.q = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
     z.k = make_plan(es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged);
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
@@ -904,7 +992,7 @@ static int join_groups(int nsplit, long n4, int most) {
 
 template <typename T, int D>
 static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
-    constexpr int T4 = sizeof(T) * D <= 256 ? 64 : 32;
+    constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
     const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R;
     use(a, z.f);
     a.part = ws;
@@ -919,7 +1007,7 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
 
 template <typename T, int D>
 static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
-    constexpr int T4 = sizeof(T) * D <= 256 ? 64 : 32;
+    constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
     const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R, keys = nbh * a.Sk;
     a.part = ws;
     use(a, z.q);
