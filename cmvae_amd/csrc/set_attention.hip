@@ -44,7 +44,7 @@ struct Args {
     float *lse, *delta, *part, *part_ml;
     const int *q_len, *k_len;
     long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, g_sb, g_ss, g_sh;   // strides in elements
-    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, ntiles, sg, fold;
+    int B, Sq, Sk, H, Hkv, G, R, causal, residual, nsplit, ntiles, sg, fold, piece;
     float scale, c;                                                                // c = scale * log2(e)
 };
 
@@ -557,6 +557,202 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
         }
 }
 
+// ------------------------------------------------------------------------------------------------ forward of few rows
+// A key head's list of at most 8 rows (one new token of grouped heads, a set's summary by one query) against many keys: the
+// keys and values are read once, and that is the time.  No LDS, no matrix instruction (32 columns of which 1 .. 8 count):
+// a row of keys lies over CL lanes, 16 bytes each, 64 / CL keys per wave and step, U steps' loads in flight; a score is the
+// sum over the CL lanes, a lane keeps its channels' sums for its keys and its own running maximum, and the waves join at the
+// end.  16-bit values meet in v_dot2 (two products per instruction): scores over channel pairs, sums over pairs of keys.
+// A workgroup takes `piece` keys; pieces of a list are joined by fwd_join_kernel.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+template <int CL>
+__device__ __forceinline__ float sum_lanes(float x) {
+    x += dpp<0xB1>(x);                            // lane ^ 1
+    x += dpp<0x4E>(x);                            // lane ^ 2
+    x += dpp<0x141>(x);                           // the other four of eight
+    if constexpr (CL >= 16) x += dpp<0x140>(x);   // the other eight of sixteen
+    if constexpr (CL >= 32) x += __shfl_xor(x, 16);
+    return x;
+}
+__device__ __forceinline__ float dot2(unsigned a, unsigned b, float c, __bf16) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+}
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float dot2(unsigned a, unsigned b, float c, _Float16) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x, y}, T2));
+}
+
+template <typename T, int D, int R>
+__global__ __launch_bounds__(256) void fwd_rows_kernel(Args a) {
+    constexpr int CL = D * sizeof(T) / 16, KP = 64 / CL, E = 16 / sizeof(T), U = 4;
+    constexpr int STEP = U * KP;                                    // keys per wave and round
+    __shared__ float sm[4][R], sl[4][R];
+    __shared__ float so[4][R][D];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ch = lane % CL, kg = lane / CL;
+    const int nbh = a.B * a.Hkv, bh = (int)blockIdx.x % nbh, split = (int)blockIdx.x / nbh;
+    const int b = bh / a.Hkv, kh = bh - b * a.Hkv;
+    int ql, kl;
+    lens(a, b, ql, kl);
+    const int rv = a.G * ql, off = kl - ql;
+    const long es = sizeof(T);
+    const int k0 = split * a.piece, k1 = min(kl, k0 + a.piece);
+    const char* kb = a.k + (b * a.k_sb + kh * a.k_sh) * es + ch * 16;
+    const char* vb = a.v + (b * a.v_sb + kh * a.v_sh) * es + ch * 16;
+    u32x4 q[R];
+    int last[R];                                                    // row r's keys end here
+    float m[R], l[R], acc[R][E];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        q[r] = u32x4{0, 0, 0, 0};
+        last[r] = 0;
+        if (r < rv) {
+            const int g = r / ql, pos = r - g * ql;
+            q[r] = *reinterpret_cast<const u32x4*>(a.q + (b * a.q_sb + pos * a.q_ss + (kh * a.G + g) * a.q_sh) * es + ch * 16);
+            last[r] = a.causal ? min(kl, pos + off + 1) : kl;
+        }
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
+    }
+    for (int kc = k0 + w * STEP; kc < k1; kc += 4 * STEP) {
+        u32x4 kv[U], vv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = kc + u * KP + kg;
+            kv[u] = vv[u] = u32x4{0, 0, 0, 0};
+            if (key < k1) {
+                kv[u] = *reinterpret_cast<const u32x4*>(kb + key * a.k_ss * es);
+                vv[u] = *reinterpret_cast<const u32x4*>(vb + key * a.v_ss * es);
+            }
+        }
+        float p[R][U];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mx = m[r];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float s = 0.f;
+                if constexpr (std::is_same<T, float>::value) {
+                    const f32x4 x = __builtin_bit_cast(f32x4, q[r]), y = __builtin_bit_cast(f32x4, kv[u]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s = fmaf(x[e], y[e], s);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s = dot2(q[r][e], kv[u][e], s, T());
+                }
+                s = sum_lanes<CL>(s);
+                p[r][u] = kc + u * KP + kg < last[r] ? s : -INFINITY;
+                mx = fmaxf(mx, p[r][u] * a.c);
+            }
+            const float mu = mx == -INFINITY ? 0.f : mx, al = exp2_raw(m[r] - mu), sub = mu - p_shift<T>();
+            m[r] = mx;
+            float ps = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                p[r][u] = exp2_raw(fmaf(p[r][u], a.c, -sub));
+                ps += p[r][u];
+            }
+            l[r] = fmaf(l[r], al, ps);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] *= al;
+        }
+        if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const f32x4 y = __builtin_bit_cast(f32x4, vv[u]);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(p[r][u], y[e], acc[r][e]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u += 2) {                        // two keys' values at one channel beside each other
+                unsigned y[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[2 * e] = __builtin_amdgcn_perm(vv[u + 1][e], vv[u][e], 0x05040100);
+                    y[2 * e + 1] = __builtin_amdgcn_perm(vv[u + 1][e], vv[u][e], 0x07060302);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const unsigned pp = pack2<T>(p[r][u], p[r][u + 1]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[r][e] = dot2(pp, y[e], acc[r][e], T());
+                }
+            }
+        }
+    }
+    // the wave's key groups meet, then the waves
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float mx = m[r];
+#pragma unroll
+        for (int o = CL; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        const float f = exp2_raw(m[r] - (mx == -INFINITY ? 0.f : mx));
+        float ls = l[r] * f;
+#pragma unroll
+        for (int o = CL; o < 64; o <<= 1) ls += __shfl_xor(ls, o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float x = acc[r][e] * f;
+#pragma unroll
+            for (int o = CL; o < 64; o <<= 1) x += __shfl_xor(x, o);
+            if (kg == 0) so[w][r][ch * E + e] = x;
+        }
+        if (lane == 0) {
+            sm[w][r] = mx;
+            sl[w][r] = ls;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.R * (D / 4); i += 256) {
+        const int r = i / (D / 4), d4 = i - r * (D / 4);
+        const Row me = row_of(a, ql, r);
+        float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        float ls = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float f = exp2_raw(sm[j][r] - mu);
+            ls = fmaf(sl[j][r], f, ls);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&so[j][r][d4 * 4]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+        }
+        const long hrow = ((long)b * a.H + kh * a.G + me.g) * a.Sq + me.pos;
+        if (a.nsplit > 1) {
+            const long prow = (long)split * nbh * a.R + hrow;
+            if (d4 == 0) {
+                a.part_ml[prow * 2] = mx;
+                a.part_ml[prow * 2 + 1] = ls;
+            }
+            if (mx != -INFINITY) *reinterpret_cast<f32x4*>(a.part + prow * D + d4 * 4) = o;
+            continue;
+        }
+        const bool ok = me.ok && ls != 0.f;
+        if (d4 == 0 && a.lse) a.lse[hrow] = ok ? mx - p_shift<T>() + log2f(ls) : INFINITY;
+        const float inv = ok ? 1.f / ls : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = ok ? o[e] * inv : 0.f;
+        const long at = ((((long)b * a.Sq + me.pos) * a.H + kh * a.G + me.g) * D + d4 * 4) * es;
+        if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
+        if (a.residual && me.ok)
+            o += load4<T>(a.q + (b * a.q_sb + me.pos * a.q_ss + (kh * a.G + me.g) * a.q_sh + d4 * 4) * es);
+        store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
+    }
+}
+
 // Joins the splits of a row: D / 4 lanes per row times SG groups that share its splits out (SG from the host: few rows of
 // many splits would otherwise be a long walk on a handful of lanes; 16 rows of 50 splits took 24 us that way).
 template <typename T, int D>
@@ -575,7 +771,9 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
         const float mu = m == -INFINITY ? 0.f : m;
         for (int s = sg; s < a.nsplit; s += a.sg) {
             const long at = s * rows + row;
-            const float wgt = exp2_raw(a.part_ml[at * 2] - mu);
+            const float pm = a.part_ml[at * 2];
+            if (pm == -INFINITY) continue;            // a piece without a valid key: its sums may not have been written
+            const float wgt = exp2_raw(pm - mu);
             l = fmaf(wgt, a.part_ml[at * 2 + 1], l);
             const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + at * D + d4 * 4);
 #pragma unroll
@@ -757,7 +955,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------ backward, key side
 // NW waves of 32 keys; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
 template <typename T, int D, int NW, int RT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 ? 2 : 1) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof(T) * D == 256 && sizeof(T) == 4) ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = Elem<T>::P * RT * pitch<D>(), BUF = 2 * TB + RT * 8;
     const Place pl = place<NW * 32, true>(a);
@@ -913,7 +1111,7 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
 
 // ------------------------------------------------------------------------------------------------ launches
 struct Plan {
-    int nw, tile, ntiles, nsplit, occ;              // waves per workgroup, contraction rows per tile, tiles of own rows
+    int nw, tile, ntiles, nsplit, occ, piece;       // waves per workgroup, contraction rows per tile, tiles of own rows
     size_t lds;
 };
 
@@ -923,6 +1121,7 @@ struct Plan {
 // are of very different length, and half again as much where lengths will leave some without work.
 static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats, int occ, bool causal, bool ragged) {
     Plan p;
+    p.piece = 0;
     p.occ = occ;
     const long wg4 = nbh * ((rows + 127) / 128), cus = compute_units();
     p.nw = wg4 >= cus ? 4 : 1;
@@ -943,6 +1142,21 @@ static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats,
     return p;
 }
 
+// Few rows: four waves per workgroup, at least two rounds of 16-byte loads each per piece, eight workgroups per unit (of padded lists some have no keys: 4 82 us, 8 76, 16 79 at 16 lists of up to 8191 keys x 8 heads of 128).
+static Plan rows_plan(int esize, int D, long nbh, int len) {
+    Plan p = {4, 0, 1, 1, 4, 0, 0};
+    const int round = 4 * 4 * (64 / (D * esize / 16));           // keys per round of a workgroup
+    const long want = 8L * compute_units();
+    long ns = (want + nbh - 1) / nbh;
+    const long most = (len + 2 * round - 1) / (2 * round);
+    if (ns > most) ns = most;
+    if (ns < 1) ns = 1;
+    if (ns > 64) ns = 64;
+    p.piece = (int)((((len + ns - 1) / ns) + round - 1) / round * round);
+    p.nsplit = len > 0 ? (len + p.piece - 1) / p.piece : 1;
+    return p;
+}
+
 static size_t esize_of(int dtype) { return dtype == CMVAE_F32 ? 4 : 2; }
 
 struct Sizes {
@@ -955,7 +1169,7 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const long nbh = (long)d.B * d.Hkv;
     const int R = G * d.Sq;
     const bool causal = d.causal != 0, ragged = d.q_len || d.k_len;
-    z.f = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
+    z.f = R <= 8 ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
     z.q = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
     z.k = make_plan(es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged);
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
@@ -980,6 +1194,7 @@ static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a,
 static void use(Args& a, const Plan& p) {
     a.ntiles = p.ntiles;
     a.nsplit = p.nsplit;
+    a.piece = p.piece;
     a.fold = p.occ >= 2 ? compute_units() : 1 << 29;
 }
 
@@ -998,7 +1213,12 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
     a.part = ws;
     a.part_ml = ws + (size_t)a.nsplit * rows * D;
     const long blocks = nbh * a.ntiles * a.nsplit;
-    int e = z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
+    const char* what = "set_attention fwd_rows_kernel";
+    int e = a.R == 1 ? launch(fwd_rows_kernel<T, D, 1>, blocks, 256, 0, a, stream, what)
+            : a.R == 2 ? launch(fwd_rows_kernel<T, D, 2>, blocks, 256, 0, a, stream, what)
+            : a.R <= 4 ? launch(fwd_rows_kernel<T, D, 4>, blocks, 256, 0, a, stream, what)
+            : a.R <= 8 ? launch(fwd_rows_kernel<T, D, 8>, blocks, 256, 0, a, stream, what)
+            : z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
                         : launch(fwd_kernel<T, D, 1, 32>, blocks, 64, z.f.lds, a, stream, "set_attention fwd_kernel");
     if (e || a.nsplit == 1) return e;
     a.sg = join_groups(a.nsplit, rows * (D / 4), 256 / (D / 4));
