@@ -279,30 +279,40 @@ __device__ __forceinline__ f32x4 load4(const char* p) {
 }
 
 // ---- tiles of ROWS rows through registers into LDS: requested while the previous tile is used -----------------------
+// A thread's pieces lie STEP rows apart, so their addresses are one 32-bit offset per thread on top of a scalar base (with a
+// 64-bit product per piece and tile instead, and a division per piece on the key side, dk and dv of dense 8 x 4096 x 16 heads
+// of 64 took @A@ us for @B@).
 template <typename T, int D, int ROWS, int THREADS>
 struct Stage {
     static constexpr int CPR = D * sizeof(T) / 16;               // 16-byte pieces per row
-    static constexpr int N = ROWS * CPR / THREADS;
-    static_assert(ROWS * CPR % THREADS == 0, "whole pieces per thread");
+    static constexpr int N = ROWS * CPR / THREADS, STEP = THREADS / CPR;
+    static_assert(ROWS * CPR % THREADS == 0 && THREADS % CPR == 0, "whole pieces per thread");
     u32x4 x[N];
-    // keys: consecutive rows of one tensor; rows from `end` on are zeros
-    __device__ __forceinline__ void load(const char* base, long stride_bytes, int row0, int end) {
+    __device__ __forceinline__ static unsigned offset(long stride) {
+        return (unsigned)((int)threadIdx.x / CPR * (int)stride + (int)threadIdx.x % CPR * 16);
+    }
+    // `left` rows from `base` on, the others are zeros
+    __device__ __forceinline__ void load(const char* base, long stride, unsigned off, int left) {
+        if (left >= ROWS) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = i * THREADS + threadIdx.x, row = row0 + id / CPR;
-            x[i] = u32x4{0, 0, 0, 0};
-            if (row < end) x[i] = *reinterpret_cast<const u32x4*>(base + row * stride_bytes + (id % CPR) * 16);
+            for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const u32x4*>(base + i * STEP * stride + off);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = u32x4{0, 0, 0, 0};
+                if (i * STEP + (int)threadIdx.x / CPR < left) x[i] = *reinterpret_cast<const u32x4*>(base + i * STEP * stride + off);
+            }
         }
     }
-    // query rows r0 .. of a key head's list: (head, position) = divmod(r, ql); rows from `end` = G ql on are zeros
-    __device__ __forceinline__ void load_rows(const char* base, long ss, long sh, int r0, int end, int ql) {
+    // rows of a key head's list from (g, pos) on, `left` of them to the list's end, through more than one head
+    __device__ __forceinline__ void load_across(const char* base, long ss, long sh, int g, int pos, int left, int ql) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = i * THREADS + threadIdx.x, r = r0 + id / CPR;
+            const int j = i * STEP + (int)threadIdx.x / CPR;
             x[i] = u32x4{0, 0, 0, 0};
-            if (r < end) {
-                const int g = r / ql, pos = r - g * ql;
-                x[i] = *reinterpret_cast<const u32x4*>(base + pos * ss + g * sh + (id % CPR) * 16);
+            if (j < left) {
+                const int q = (pos + j) / ql;
+                x[i] = *reinterpret_cast<const u32x4*>(base + (pos + j - q * ql) * ss + (g + q) * sh + (int)threadIdx.x % CPR * 16);
             }
         }
     }
@@ -465,10 +475,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
     float m = -INFINITY, l = 0.f;
     const int klast = a.causal ? min(kl, pos + off + 1) : kl;      // this row's keys end here
 
-    Stage<T, D, KT, NW * 64> ks, vs;
+    typedef Stage<T, D, KT, NW * 64> St;
+    St ks, vs;
+    const long ksb = a.k_ss * es, vsb = a.v_ss * es;
+    const unsigned ko = St::offset(ksb), vo = St::offset(vsb);
+    auto request = [&](int t) {
+        ks.load(kb + (long)t * KT * ksb, ksb, ko, kl - t * KT);
+        vs.load(vb + (long)t * KT * vsb, vsb, vo, kl - t * KT);
+    };
     if (t0 < t1) {
-        ks.load(kb, a.k_ss * es, t0 * KT, kl);
-        vs.load(vb, a.v_ss * es, t0 * KT, kl);
+        request(t0);
         ks.put(smem, sel);
         vs.put(smem + TB, sel);
     }
@@ -476,10 +492,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
     for (int t = t0; t < t1; ++t) {
         const char* kt = smem + ((t - t0) & 1) * 2 * TB;
         const char* vt = kt + TB;
-        if (t + 1 < t1) {
-            ks.load(kb, a.k_ss * es, (t + 1) * KT, kl);
-            vs.load(vb, a.v_ss * es, (t + 1) * KT, kl);
-        }
+        if (t + 1 < t1) request(t + 1);
         f32x16 s[KT / 32];
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) s[u] = mul_rows<T, D, KT>(kt, u * 32, qf, zero16());
@@ -878,10 +891,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
     for (int d = 0; d < D / 32; ++d) acc[d] = zero16();
     const int klast = a.causal ? min(kl, pos + off + 1) : kl;
 
-    Stage<T, D, KT, NW * 64> ks, vs;
+    typedef Stage<T, D, KT, NW * 64> St;
+    St ks, vs;
+    const long ksb = a.k_ss * es, vsb = a.v_ss * es;
+    const unsigned ko = St::offset(ksb), vo = St::offset(vsb);
+    auto request = [&](int t) {
+        ks.load(kb + (long)t * KT * ksb, ksb, ko, kl - t * KT);
+        vs.load(vb + (long)t * KT * vsb, vsb, vo, kl - t * KT);
+    };
     if (t0 < t1) {
-        ks.load(kb, a.k_ss * es, t0 * KT, kl);
-        vs.load(vb, a.v_ss * es, t0 * KT, kl);
+        request(t0);
         ks.put(smem, sel);
         vs.put(smem + TB, sel);
     }
@@ -889,10 +908,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
     for (int t = t0; t < t1; ++t) {
         const char* kt = smem + ((t - t0) & 1) * 2 * TB;
         const char* vt = kt + TB;
-        if (t + 1 < t1) {
-            ks.load(kb, a.k_ss * es, (t + 1) * KT, kl);
-            vs.load(vb, a.v_ss * es, (t + 1) * KT, kl);
-        }
+        if (t + 1 < t1) request(t + 1);
         const int k0 = t * KT;
         const bool edge = k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1);
 #pragma unroll
@@ -981,29 +997,48 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
         t1 = min(t1, t + per);
     }
     if (key0 >= kl) t = t1;
-    // the next tile of rows with a valid pair, from t on
-    auto next = [&](int t) {
-        for (; t < t1; ++t) {
-            int lo, hi;
-            if (!a.causal) break;
-            span(ql, t * RT, min(t * RT + RT, rv), lo, hi);
-            if (hi + off >= key0) break;
+    // a tile's place in the list: its first row's head and position; rows behind the head's last one are the next head's
+    struct At {
+        int t, g, pos;
+    };
+    auto step = [&](At x) {
+        ++x.t;
+        x.pos += RT;
+        while (x.pos >= ql) {
+            x.pos -= ql;
+            ++x.g;
         }
-        return t;
+        return x;
+    };
+    // the next tile of rows with a valid pair, from x on
+    auto next = [&](At x) {
+        if (a.causal)
+            while (x.t < t1 && min(x.pos + RT, ql) - 1 + off < key0 && x.pos + RT <= ql) x = step(x);
+        return x;
     };
     constexpr float unshift = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.f;
-    Stage<T, D, RT, NW * 64> qs, gs;
+    typedef Stage<T, D, RT, NW * 64> St;
+    St qs, gs;
+    const long qss = a.q_ss * es, qsh = a.q_sh * es, gss = a.g_ss * es, gsh = a.g_sh * es;
+    const unsigned qo = St::offset(qss), go = St::offset(gss);
     float st_lse = 0.f, st_dl = 0.f;
-    auto request = [&](int t) {
-        qs.load_rows(qb, a.q_ss * es, a.q_sh * es, t * RT, rv, ql);
-        gs.load_rows(gb, a.g_ss * es, a.g_sh * es, t * RT, rv, ql);
+    auto request = [&](At x) {
+        const int left = rv - x.t * RT;
+        const bool one = x.pos + min(left, RT) <= ql;             // all of one head
+        if (one) {
+            qs.load(qb + x.g * qsh + x.pos * qss, qss, qo, left);
+            gs.load(gb + x.g * gsh + x.pos * gss, gss, go, left);
+        } else {
+            qs.load_across(qb, qss, qsh, x.g, x.pos, left, ql);
+            gs.load_across(gb, gss, gsh, x.g, x.pos, left, ql);
+        }
         if (threadIdx.x < RT) {
-            const int r = t * RT + threadIdx.x;
+            const int j = threadIdx.x;
             st_lse = INFINITY;
             st_dl = 0.f;
-            if (r < rv) {
-                const int g = r / ql;
-                const long at = hrow0 + (long)g * a.Sq + (r - g * ql);
+            if (j < left) {
+                const int q = one ? 0 : (x.pos + j) / ql;
+                const long at = hrow0 + (long)(x.g + q) * a.Sq + (x.pos + j - q * ql);
                 st_lse = a.lse[at] - p_shift<T>();
                 st_dl = a.delta[at] * unshift;
             }
@@ -1017,23 +1052,24 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
             reinterpret_cast<float*>(buf + 2 * TB)[RT + threadIdx.x] = st_dl;
         }
     };
-    t = next(t);
+    At x = {t, 0, 0};
     if (t < t1) {
-        request(t);
+        x.g = t * RT / ql;
+        x.pos = t * RT - x.g * ql;
+        x = next(x);
+    }
+    if (x.t < t1) {
+        request(x);
         put(smem);
     }
     __syncthreads();
     int cur = 0;
-    while (t < t1) {
+    while (x.t < t1) {
         const char* buf = smem + cur * BUF;
-        const int tn = next(t + 1);
-        if (tn < t1) request(tn);
-        bool edge = false;
-        if (a.causal) {
-            int lo, hi;
-            span(ql, t * RT, min(t * RT + RT, rv), lo, hi);
-            edge = lo + off < key0 + NW * 32 - 1;
-        }
+        const At xn = next(step(x));
+        if (xn.t < t1) request(xn);
+        const bool across = x.pos + RT > ql;
+        const bool edge = a.causal && (across ? 0 : x.pos) + off < key0 + NW * 32 - 1;
 #pragma unroll
         for (int u = 0; u < RT / 32; ++u) {
             f32x16 s = mul_rows<T, D, RT>(buf, u * 32, kf, zero16());
@@ -1048,7 +1084,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = t * RT + u * 32 + acc_row(i, h), p = r - r / ql * ql;
+                    int p = x.pos + u * 32 + acc_row(i, h);
+                    if (across) p -= p / ql * ql;
                     if (p + off < key) s[i] = 0.f;
                 }
             }
@@ -1061,10 +1098,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
             }
             mul_cols<T, D, RT>(buf, u * 32, s, sel, dk);
         }
-        if (tn < t1) put(smem + (cur ^ 1) * BUF);
+        if (xn.t < t1) put(smem + (cur ^ 1) * BUF);
         __syncthreads();
         cur ^= 1;
-        t = tn;
+        x = xn;
     }
     if (key >= a.Sk) return;
     const long krow = ((long)pl.b * a.Sk + key) * a.Hkv + pl.kh;
@@ -1117,8 +1154,8 @@ struct Plan {
 
 // `rows` own rows in tiles of 32 per wave, `len` rows to walk; `occ` workgroups of four waves fit on a compute unit.  Four
 // waves share what they walk; where that leaves most of the card idle, one wave per workgroup.  The walk is cut into pieces,
-// which a second launch joins, until there is work for every wave slot — twice that for the causal order, whose workgroups
-// are of very different length, and half again as much where lengths will leave some without work.
+// which a second launch joins, until there is work for every wave slot — twice that for the causal order at one
+// workgroup per unit (two are dealt in pairs, see place()), and half again as much where lengths will leave some without work.
 static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats, int occ, bool causal, bool ragged) {
     Plan p;
     p.piece = 0;
@@ -1131,7 +1168,7 @@ static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats,
     const int tiles = (len + p.tile - 1) / p.tile;
     const long wg = nbh * p.ntiles;
     long want = p.nw == 4 ? cus * occ : 4 * cus;
-    if (p.nw == 4) want = causal ? 2 * want : ragged ? want + want / 2 : want;
+    if (p.nw == 4) want = causal && occ == 1 ? 2 * want : ragged ? want + want / 2 : want;
     const int least = p.nw == 4 ? 4 : 2;          // tiles per piece
     if (wg > 0 && wg < want && tiles >= 2 * least) {
         long ns = (want + wg - 1) / wg;
@@ -1250,11 +1287,11 @@ static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
     return launch(dkv_join_kernel<T, D>, (n4 * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dkv_join_kernel");
 }
 
-static bool aligned(const void* p, const int64_t* s, int dtype, int extra) {
+static bool aligned(const void* p, const int64_t* s, int dtype) {
     const int m = 16 / (int)esize_of(dtype);
     for (int i = 0; i < 3; ++i)
         if (s[i] % m || s[i] < 0) return false;
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && extra % m == 0;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s[1] < (1 << 22);       // a tile's 64 rows: 31-bit offsets
 }
 
 static int check_desc(const char* who, const cmvae_set_attn* d) {
@@ -1323,9 +1360,9 @@ extern "C" int cmvae_set_attention_fwd(const cmvae_set_attn* d, void* workspace,
     cmvae::clear_stale_error();
     if (int e = sa::check_desc("cmvae_set_attention_fwd", d)) return e;
     CMVAE_REQUIRE(d->q && d->o && (d->Sk == 0 || (d->k && d->v)), "cmvae_set_attention_fwd: NULL tensor");
-    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype, 0) && sa::aligned(d->k, d->k_stride, d->dtype, 0) &&
-                      sa::aligned(d->v, d->v_stride, d->dtype, 0) && ((uintptr_t)d->o & 15) == 0 && ((uintptr_t)d->attn & 15) == 0,
-                  "cmvae_set_attention_fwd: rows must start at multiples of 16 bytes");
+    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype) && sa::aligned(d->k, d->k_stride, d->dtype) &&
+                      sa::aligned(d->v, d->v_stride, d->dtype) && ((uintptr_t)d->o & 15) == 0 && ((uintptr_t)d->attn & 15) == 0,
+                  "cmvae_set_attention_fwd: rows must start at multiples of 16 bytes and lie under 2^22 elements apart");
     const sa::Sizes z = sa::sizes_of(*d);
     CMVAE_REQUIRE(z.fwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.fwd),
                   "cmvae_set_attention_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, z.fwd);
@@ -1339,10 +1376,10 @@ extern "C" int cmvae_set_attention_bwd(const cmvae_set_attn* d, void* workspace,
     CMVAE_REQUIRE(d->q && d->dO && d->lse && d->delta && d->dq && (d->residual ? (const void*)d->attn : d->o) &&
                       (d->Sk == 0 || (d->k && d->v && d->dk && d->dv)),
                   "cmvae_set_attention_bwd: NULL tensor");
-    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype, 0) && sa::aligned(d->k, d->k_stride, d->dtype, 0) &&
-                      sa::aligned(d->v, d->v_stride, d->dtype, 0) && sa::aligned(d->dO, d->dO_stride, d->dtype, 0) &&
+    CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype) && sa::aligned(d->k, d->k_stride, d->dtype) &&
+                      sa::aligned(d->v, d->v_stride, d->dtype) && sa::aligned(d->dO, d->dO_stride, d->dtype) &&
                       (((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv | (uintptr_t)d->o | (uintptr_t)d->attn) & 15) == 0,
-                  "cmvae_set_attention_bwd: rows must start at multiples of 16 bytes");
+                  "cmvae_set_attention_bwd: rows must start at multiples of 16 bytes and lie under 2^22 elements apart");
     const sa::Sizes z = sa::sizes_of(*d);
     CMVAE_REQUIRE(z.bwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bwd),
                   "cmvae_set_attention_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, z.bwd);

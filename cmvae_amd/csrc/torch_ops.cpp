@@ -86,11 +86,11 @@ variable_list once(variable_list grads, const char* what) {
 }
 
 // ------------------------------------------------------------------------------------------------ set attention
-// t with adjacent channels and rows that start at multiples of 16 bytes (a copy if it has not)
+// t with adjacent channels and rows that start at multiples of 16 bytes under 2^22 elements apart (a copy if it has not)
 Tensor rows16(const Tensor& t) {
     const int64_t per = 16 / t.element_size();
     auto s = t.strides();
-    if (s[3] != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || s[0] % per || s[1] % per || s[2] % per)
+    if (s[3] != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || s[0] % per || s[1] % per || s[2] % per || s[1] >= (1 << 22))
         return t.clone(at::MemoryFormat::Contiguous);
     return t;
 }

@@ -295,7 +295,7 @@ int cmvae_attention_qkv_bwd(const float* QKV, const float* lse, const float* dO,
  *   s_ij = scale q_i . k_j;  valid (i, j): i < q_len[b], j < k_len[b] and, if causal, j <= i + k_len[b] - q_len[b];
  *   o_i = softmax over the valid j (no valid j: zeros) . v  (+ q_i if residual);  rows i >= q_len[b] of o are zeros.
  * q, dO [B,Sq,H,D] and k, v [B,Sk,Hkv,D] with strides {batch, row, head} in elements (channels are adjacent, rows start
- * at multiples of 16 bytes); D 64 or 128, H a multiple of Hkv (query head h reads key head h / (H / Hkv)).  o, attn, dq
+ * at multiples of 16 bytes and lie under 2^22 elements apart); D 64 or 128, H a multiple of Hkv (query head h reads key head h / (H / Hkv)).  o, attn, dq
  * [B,Sq,H,D] and dk, dv [B,Sk,Hkv,D] are dense.  q_len, k_len: int32 [B] or NULL (all rows), clamped to the tensors.
  * Values of rows behind a length are not read.  lse, delta: fp32 [B,H,Sq].  Forward: lse may be NULL; attn, if not NULL,
  * receives o without the residual.  Backward: reads o (residual: attn) and lse of the forward, writes delta (scratch),
