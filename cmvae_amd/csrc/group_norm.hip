@@ -77,23 +77,38 @@ __device__ __forceinline__ void put_param(void* p, int type, int c, double v) {
     else ((_Float16*)p)[c] = (_Float16)(float)v;
 }
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-    switch (act) {
-        case 1: return z > 0.f ? z : (z != z ? z : 0.f);
-        case 2: return elu1(z);
-        case 3: return z / (1.f + __expf(-z));
-        default: return z;
+// 1 / (1 + e^-z); the reciprocal to 1 ulp (a division is ten instructions of the backward's forty per value)
+__device__ __forceinline__ float sigmoid1(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+
+// z -> act(z) of a thread's vector: one branch per vector
+template <int V>
+__device__ __forceinline__ void activate(float (&z)[V], int act) {
+    if (act == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = z[j] > 0.f ? z[j] : (z[j] != z[j] ? z[j] : 0.f);
+    } else if (act == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = elu1(z[j]);
+    } else if (act == 3) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] *= sigmoid1(z[j]);
     }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case 1: return z > 0.f ? 1.f : 0.f;
-        case 2: return z > 0.f ? 1.f : __expf(z);
-        case 3: {
-            const float s = 1.f / (1.f + __expf(-z));
-            return s * fmaf(z, 1.f - s, 1.f);
+// d -> d act'(z)
+template <int V>
+__device__ __forceinline__ void slope(const float (&z)[V], float (&d)[V], int act) {
+    if (act == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = z[j] > 0.f ? d[j] : 0.f;
+    } else if (act == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = z[j] > 0.f ? d[j] : d[j] * __expf(z[j]);
+    } else if (act == 3) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float s = sigmoid1(z[j]);
+            d[j] *= s * fmaf(z[j], 1.f - s, 1.f);
         }
-        default: return 1.f;
     }
 }
 
@@ -117,6 +132,24 @@ __device__ __forceinline__ void load_channels(const Args& a, const float4* st, i
         k.w[j] = param(a.w, a.wtype, c0 + j, 1.f);
         k.b[j] = param(a.b, a.wtype, c0 + j, 0.f);
     }
+}
+
+// x -> xhat, d = dy -> dz
+template <int V>
+__device__ __forceinline__ void backward_of(const Channel<V>& k, int act, float (&x)[V], float (&d)[V]) {
+    float z[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        x[j] = (x[j] - k.mh[j] - k.ml[j]) * k.rs[j];
+        z[j] = fmaf(x[j], k.w[j], k.b[j]);
+    }
+    slope<V>(z, d, act);
+}
+template <int V>
+__device__ __forceinline__ void forward_of(const Channel<V>& k, int act, float (&x)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = fmaf((x[j] - k.mh[j] - k.ml[j]) * k.rs[j], k.w[j], k.b[j]);
+    activate<V>(x, act);
 }
 
 // ------------------------------------------------------------------------------------------------ resident
@@ -190,9 +223,7 @@ __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
         if (p < a.P) {
             float v[V];
             unpack<T, V>(hold[i], v);
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                v[j] = act_fwd(fmaf((v[j] - k.mh[j] - k.ml[j]) * k.rs[j], k.w[j], k.b[j]), a.act);
+            forward_of<V>(k, a.act, v);
             *reinterpret_cast<TV*>(y + (long)p * a.C) = pack<T, V>(v);
         }
     }
@@ -233,12 +264,11 @@ __global__ __launch_bounds__(THREADS) void bwd_resident_kernel(Args a) {
             float v[V], d[V];
             unpack<T, V>(hx[i], v);
             unpack<T, V>(hg[i], d);
+            backward_of<V>(k, a.act, v, d);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
-                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
-                s1[j] += dz;
-                s2[j] = fmaf(dz, xh, s2[j]);
+                s1[j] += d[j];
+                s2[j] = fmaf(d[j], v[j], s2[j]);
             }
         }
     }
@@ -285,12 +315,9 @@ __global__ __launch_bounds__(THREADS) void bwd_resident_kernel(Args a) {
             float v[V], d[V];
             unpack<T, V>(hx[i], v);
             unpack<T, V>(hg[i], d);
+            backward_of<V>(k, a.act, v, d);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
-                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
-                v[j] = k.rs[j] * (fmaf(dz, k.w[j], -m1[j]) - xh * m2[j]);
-            }
+            for (int j = 0; j < V; ++j) v[j] = k.rs[j] * (fmaf(d[j], k.w[j], -m1[j]) - v[j] * m2[j]);
             *reinterpret_cast<TV*>(dx + (long)p * a.C) = pack<T, V>(v);
         }
     }
@@ -356,23 +383,36 @@ __global__ __launch_bounds__(256) void fwd_sums_kernel(Args a) {
     }
 }
 
-// one wave per (sample, group)
-__global__ __launch_bounds__(64) void fwd_finish_kernel(Args a) {
-    const long ng = blockIdx.x;
-    const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
-    double u = 0.0, v = 0.0;
-    const int items = a.pc * a.Cg;
-    for (int i = threadIdx.x; i < items; i += 64) {
-        const int pc = i / a.Cg, c = i - pc * a.Cg;
-        const double2 s = a.part[((long)n * a.pc + pc) * a.C + g * a.Cg + c];
-        u += s.x;
-        v += s.y;
-    }
+// sums u, v over the 256 threads of a workgroup, in thread 0
+__device__ __forceinline__ void block_sum(double& u, double& v) {
+    __shared__ double2 red[4];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         u += __shfl_xor(u, o);
         v += __shfl_xor(v, o);
     }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_double2(u, v);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 1; i < 4; ++i) {
+            u += red[i].x;
+            v += red[i].y;
+        }
+}
+
+// one workgroup per (sample, group)
+__global__ __launch_bounds__(256) void fwd_finish_kernel(Args a) {
+    const long ng = blockIdx.x;
+    const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
+    double u = 0.0, v = 0.0;
+    const int items = a.pc * a.Cg;
+    for (int i = threadIdx.x; i < items; i += 256) {
+        const int pc = i / a.Cg, c = i - pc * a.Cg;
+        const double2 s = a.part[((long)n * a.pc + pc) * a.C + g * a.Cg + c];
+        u += s.x;
+        v += s.y;
+    }
+    block_sum(u, v);
     if (threadIdx.x == 0) a.stats[ng] = make_stats(u, v, (double)a.P * a.Cg, a.eps);
 }
 
@@ -389,8 +429,7 @@ __global__ __launch_bounds__(256) void fwd_apply_kernel(Args a) {
     for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
         float v[V];
         unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = act_fwd(fmaf((v[j] - k.mh[j] - k.ml[j]) * k.rs[j], k.w[j], k.b[j]), a.act);
+        forward_of<V>(k, a.act, v);
         *reinterpret_cast<TV*>(y + (long)p * a.C) = pack<T, V>(v);
     }
 }
@@ -413,12 +452,11 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
             float v[V], d[V];
             unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
             unpack<T, V>(*reinterpret_cast<const TV*>(dy + p * a.g_sp), d);
+            backward_of<V>(k, a.act, v, d);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
-                const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
-                s1[j] += dz;
-                s2[j] = fmaf(dz, xh, s2[j]);
+                s1[j] += d[j];
+                s2[j] = fmaf(d[j], v[j], s2[j]);
             }
         }
     }
@@ -438,23 +476,19 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
     }
 }
 
-__global__ __launch_bounds__(64) void bwd_finish_kernel(Args a) {
+__global__ __launch_bounds__(256) void bwd_finish_kernel(Args a) {
     const long ng = blockIdx.x;
     const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
     double u = 0.0, v = 0.0;
     const int items = a.pc * a.Cg;
-    for (int i = threadIdx.x; i < items; i += 64) {
+    for (int i = threadIdx.x; i < items; i += 256) {
         const int pc = i / a.Cg, c = g * a.Cg + i - pc * a.Cg;
         const float2 s = a.bpart[((long)n * a.pc + pc) * a.C + c];
         const double w = (double)param(a.w, a.wtype, c, 1.f);
         u += w * (double)s.x;
         v += w * (double)s.y;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        u += __shfl_xor(u, o);
-        v += __shfl_xor(v, o);
-    }
+    block_sum(u, v);
     const double m = (double)a.P * a.Cg;
     if (threadIdx.x == 0) a.means[ng] = make_float2((float)(u / m), (float)(v / m));
 }
@@ -481,12 +515,9 @@ __global__ __launch_bounds__(256) void bwd_apply_kernel(Args a) {
         float v[V], d[V];
         unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
         unpack<T, V>(*reinterpret_cast<const TV*>(dy + p * a.g_sp), d);
+        backward_of<V>(k, a.act, v, d);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float xh = (v[j] - k.mh[j] - k.ml[j]) * k.rs[j];
-            const float dz = d[j] * act_slope(fmaf(xh, k.w[j], k.b[j]), a.act);
-            v[j] = k.rs[j] * (fmaf(dz, k.w[j], -m1[j]) - xh * m2[j]);
-        }
+        for (int j = 0; j < V; ++j) v[j] = k.rs[j] * (fmaf(d[j], k.w[j], -m1[j]) - v[j] * m2[j]);
         *reinterpret_cast<TV*>(dx + (long)p * a.C) = pack<T, V>(v);
     }
 }
@@ -594,7 +625,7 @@ static int run_fwd(Args a, const Plan& p, void* stream) {
     }
     const long blocks = (long)a.N * a.pc * a.cc;
     if (int e = launch(fwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_sums_kernel")) return e;
-    if (int e = launch(fwd_finish_kernel, (long)a.N * a.G, 64, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
+    if (int e = launch(fwd_finish_kernel, (long)a.N * a.G, 256, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
     return launch(fwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_apply_kernel");
 }
 
@@ -613,7 +644,7 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
     } else {
         const long blocks = (long)a.N * a.pc * a.cc;
         if ((e = launch(bwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_sums_kernel"))) return e;
-        if ((e = launch(bwd_finish_kernel, (long)a.N * a.G, 64, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
+        if ((e = launch(bwd_finish_kernel, (long)a.N * a.G, 256, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
         e = launch(bwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_apply_kernel");
     }
     if (e || (!a.dw && !a.db)) return e;
