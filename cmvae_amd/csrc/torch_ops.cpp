@@ -77,12 +77,17 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// gradients that cannot be differentiated again say so when that is tried
-variable_list once(variable_list grads, const char* what) {
+// Gradients that cannot be differentiated again say so when that is tried: under create_graph they get a node that throws,
+// between them and what they depend on.
+variable_list once(variable_list grads, const variable_list& of, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
+    const size_t n = grads.size();
+    grads.insert(grads.end(), of.begin(), of.end());
     auto err = std::make_shared<torch::autograd::DelayedError>(
         std::string("cmvae_amd ") + what + ": differentiable once; its gradient was differentiated", (int64_t)grads.size());
-    return (*err)(std::move(grads));
+    variable_list out = (*err)(std::move(grads));
+    out.resize(n);
+    return out;
 }
 
 // ------------------------------------------------------------------------------------------------ set attention
@@ -175,7 +180,7 @@ class SetAttention : public torch::autograd::Function<SetAttention> {
                 check(lib.sa_bwd(&d, ptr(ws), n, stream_of(q)), "cmvae_set_attention_bwd");
             }
         }
-        variable_list out = once({dq, dk, dv}, "set_attention");
+        variable_list out = once({dq, dk, dv}, {g[0], q, k, v}, "set_attention");
         out.resize(9);
         return out;
     }
@@ -294,7 +299,7 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
                 check(lib.gn_bwd(&d, ptr(ws), n, stream_of(x)), "cmvae_group_norm_bwd");
             }
         }
-        variable_list out = once({dx, dw, db}, "group_norm_act");
+        variable_list out = once({dx, dw, db}, {g[0], x, w, b}, "group_norm_act");
         return {out[0], Tensor(), out[1], out[2], Tensor(), Tensor(), Tensor()};
     }
 };

@@ -43,6 +43,9 @@ def build_parser(variant):
     p.add_argument('--graph-step', choices=('auto', 'on', 'off'), default='auto',
                    help='replay the training step from a HIP graph (new; auto: the feature variants in a single '
                         'process, whose step is bound by the host\'s launch rate; same arithmetic as the eager step)')
+    p.add_argument('--optimizer', choices=('adam', 'adamw', 'adamw8'), default='adam',
+                   help='adam: the reference\'s (weight decay as L2 in the gradient); adamw: decoupled weight decay; adamw8: '
+                        'the same with its states in 8 bits (new)')
     p.add_argument('--eval-streams', type=int, default=8,
                    help='HIP streams the independent prediction calls of an evaluation are dealt to (new; 1 = the '
                         'reference\'s sequential loop, same results)')

@@ -16,6 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import dist as _dist
+from .attention import set_attention as _set_attention
 from .linear import linear as _linear, causal_mlp as _causal_mlp, attention as _attention, \
     self_attention as _self_attention
 
@@ -89,7 +90,19 @@ class MAB(nn.Module):
         self.fc_v = nn.Linear(dim_K, dim_V)
         self.fc_o = nn.Linear(dim_V, dim_V)
 
-    def forward(self, Q, K):
+    def forward(self, Q, K, q_len=None, k_len=None):
+        """Q [B, Sq, dim], K [B, Sk, dim].  q_len, k_len (int32 [B]): how many rows of each episode count, for a batch of
+        sets padded to one size — rows behind a length (any finite values) are not attended to, their own results mean nothing, and the
+        parameters' gradients are those of the sets alone as long as no loss reads such results.  Sets of more than 1024
+        rows, unequal ones and padded ones run on `set_attention`, the others as before."""
+        if q_len is not None or k_len is not None or Q.shape[1:-1] != K.shape[1:-1] or \
+                (Q.dim() == 3 and Q.shape[1] > 1024):
+            heads = (self.num_heads, 64)
+            o = _set_attention(_linear(Q, self.fc_q.weight, self.fc_q.bias).unflatten(-1, heads),
+                               _linear(K, self.fc_k.weight, self.fc_k.bias).unflatten(-1, heads),
+                               _linear(K, self.fc_v.weight, self.fc_v.bias).unflatten(-1, heads),
+                               scale=1.0 / math.sqrt(self.dim_V), q_len=q_len, k_len=k_len, residual=True).flatten(-2)
+            return o + _linear(o, self.fc_o.weight, self.fc_o.bias, 'relu')
         if Q is K and Q.dim() == 3 and Q.shape[0] * Q.shape[1] > 0:
             # self-attention: the three projections read the same rows -> one GEMM over the stacked weights
             o = _self_attention(Q, self.fc_q.weight, self.fc_q.bias, self.fc_k.weight, self.fc_k.bias,
@@ -108,8 +121,9 @@ class SAB(nn.Module):
         super().__init__()
         self.mab = MAB(dim_in, dim_in, dim_out, num_heads, ln=ln)
 
-    def forward(self, X):
-        return self.mab(X, X)
+    def forward(self, X, lens=None):
+        """X [B, S, dim]; lens (int32 [B]): the rows of each set that count (MAB.forward)."""
+        return self.mab(X, X, lens, lens)
 
 
 class LocallyConnected(nn.Module):

@@ -25,6 +25,7 @@ from .data import EpisodeData, TrainStream
 from .graph_step import GraphedStep
 from .linear import FlatAdam
 from .model import OmniglotGMVAE, FeatureGMVAE
+from .optim import AdamW
 from .pipeline import PredictionPipeline
 
 # (h_lambda, h_c, a_lambda) and the shots validated after every epoch, per variant
@@ -68,7 +69,7 @@ class Trainer(object):
         self.input_shape = self.data.input_shape
         self.model = self._new_model()
         self.flat = cdist.FlatGrads(self.model.parameters()).overlap_tail(self.model.tail_param_count())
-        self.optimizer = FlatAdam(self.flat, lr=args.lr, weight_decay=args.weight_decay)
+        self.optimizer = self._new_optimizer()
         self.seeds = cdist.SeedUploader((self.local_batch, args.way), self.device)
         self._graphed = None
         self._pipe = None                        # the evaluation pipeline (streams + captured graphs), built once
@@ -87,6 +88,15 @@ class Trainer(object):
         else:
             m = FeatureGMVAE(input_shape=self.input_shape, linear=self.variant == 'mimgnet', **kw)
         return m.to(self.device)
+
+    def _new_optimizer(self):
+        """--optimizer: adam (the reference's: L2 in the gradient), adamw (decoupled weight decay), adamw8 (the same with
+        states in 8 bits)."""
+        a = self.args
+        kind = getattr(a, 'optimizer', 'adam')
+        if kind == 'adam':
+            return FlatAdam(self.flat, lr=a.lr, weight_decay=a.weight_decay)
+        return AdamW(self.flat, lr=a.lr, weight_decay=a.weight_decay, state_bits={'adamw': 32, 'adamw8': 8}[kind])
 
     def _log(self, rec):
         if self.rank == 0:
@@ -186,7 +196,7 @@ class Trainer(object):
         self.model = self._new_model()
         self.model.load_state_dict(state['state_dict'])
         self.flat = cdist.FlatGrads(self.model.parameters()).overlap_tail(self.model.tail_param_count())
-        self.optimizer = FlatAdam(self.flat, lr=self.args.lr, weight_decay=self.args.weight_decay)
+        self.optimizer = self._new_optimizer()
         self._graphed = None                     # graphs of the previous model's buffers are void
         self._pipe = None
         if resume_optimizer and 'optimizer' in state:
