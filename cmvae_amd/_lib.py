@@ -43,7 +43,7 @@ class SetAttnDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ('dtype', 'B', 'Sq', 'Sk', 'H', 'Hkv', 'D', 'causal', 'residual')] + \
                [('scale', c_float)] + [(n, c_void_p) for n in ('q', 'k', 'v', 'dO')] + \
                [(n, c_int64 * 3) for n in ('q_stride', 'k_stride', 'v_stride', 'dO_stride')] + \
-               [(n, c_void_p) for n in ('q_len', 'k_len', 'o', 'attn', 'lse', 'delta', 'dq', 'dk', 'dv')]
+               [(n, c_void_p) for n in ('q_len', 'k_len', 'o', 'attn', 'attn_low', 'lse', 'delta', 'dq', 'dk', 'dv')]
 
 
 class GroupNormDesc(ctypes.Structure):

@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
         load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
         const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
         const T* dy = (const T*)a.dy + q.n * a.g_sn + q.c0;
-#pragma unroll 4
+#pragma unroll 2
         for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
             float v[V], d[V];
             unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256) void bwd_apply_kernel(Args a) {
     const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
     const T* dy = (const T*)a.dy + q.n * a.g_sn + q.c0;
     T* dx = (T*)a.dx + (long)q.n * a.P * a.C + q.c0;
-#pragma unroll 4
+#pragma unroll 2
     for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
         float v[V], d[V];
         unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);

@@ -103,7 +103,7 @@ __device__ __forceinline__ void put4(void* base, long i, long n, bool whole, con
 }
 
 __device__ __forceinline__ float update(float p, float m, float v, const Consts& c) {
-    return p * c.decay - c.step * (m / (sqrtf(v) * c.rc2 + c.eps));
+    return p * c.decay - c.step * (m * __builtin_amdgcn_rcpf(sqrtf(v) * c.rc2 + c.eps));      // the reciprocal to 1 ulp
 }
 
 // ------------------------------------------------------------------------------------------------ states in 32 bits
@@ -149,15 +149,21 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Table t, Hyper h, float* m
 }
 
 // ------------------------------------------------------------------------------------------------ states in 8 bits
-__device__ __forceinline__ double max16(double x) {          // over the 16 lanes of a block of 256 values
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) x = fmax(x, __shfl_xor(x, o));
-    return x;
+// over the 16 lanes of a block of 256 values: lane ^ 1, lane ^ 2, the other four of eight, the other eight
+template <int CTRL>
+__device__ __forceinline__ double max_dpp(double x) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, 0xf, 0xf, false);
+    return fmax(x, __hiloint2double(hi, lo));
+}
+__device__ __forceinline__ double max16(double x) {
+    return max_dpp<0x140>(max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(x))));
 }
 
 __device__ __forceinline__ float decode_v(int code) {
-    const float x = __int_as_float((code + 768) << 20);
-    return code == 0 ? 0.f : code == 255 ? INFINITY : x;
+    float x = __int_as_float((code + 768) << 20);
+    x = code == 0 ? 0.f : x;
+    return code == 255 ? INFINITY : x;
 }
 
 // x rounded to e4m3's grid (quantum 2^(e - 3), e the exponent, at least -6), as a float: adding 1.5 * 2^52 quanta makes
@@ -170,11 +176,14 @@ __device__ __forceinline__ float round_m(double x) {
     return (hi & 0x7ff00000) == 0x7ff00000 ? __int_as_float(0x7fc00000) : r;
 }
 
-// x >= 0 -> code, to nearest even on the fp64 bits (the low word only as "more than a tie")
-__device__ __forceinline__ int round_v(double x) {
-    const int hi = __double2hiint(x) | (__double2loint(x) != 0);
-    const int r = ((hi + 0xffff + ((hi >> 17) & 1)) >> 17) - (1023 - 31) * 8;
-    return x > 0.0 ? min(max(r, 1), 254) : (x == 0.0 ? 0 : 255);
+// x >= 0 -> code, to nearest even on the fp64 bits (the low word only as "more than a tie"); no branch here nor where it is
+// used: sixteen of them per thread cost more than what they skip
+__device__ __forceinline__ int round_v(double x, bool finite) {
+    const int hi = __double2hiint(x) | (__double2loint(x) != 0 ? 1 : 0);
+    int r = ((hi + 0xffff + ((hi >> 17) & 1)) >> 17) - (1023 - 31) * 8;
+    r = min(max(r, 1), 254);
+    r = x > 0.0 ? r : 0;
+    return finite ? r : 255;
 }
 
 __device__ __forceinline__ double moment(double b, double x, double y) {
@@ -243,9 +252,9 @@ __device__ __forceinline__ void step8(const Table& t, int k, const Hyper& h, int
         int vc = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            r[j] = fabs(m[q][j]) <= 3.4028234663852886e38 ? round_m(over(m[q][j], nm, im)) : __int_as_float(0x7fc00000);
+            r[j] = round_m(over(m[q][j], nm, im));                // not finite: over() makes NaN of it
             const double vv = v[q][j];
-            vc |= (vv <= 3.4028234663852886e38 ? round_v(over(vv, nv, iv)) : 255) << (8 * j);
+            vc |= round_v(over(vv, nv, iv), vv <= 3.4028234663852886e38) << (8 * j);
             p[q][j] = update(p[q][j], (float)m[q][j], (float)vv, c);
         }
         int mc = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);

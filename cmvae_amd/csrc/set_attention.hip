@@ -39,8 +39,8 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
-    const char *q, *k, *v, *doo, *att;
-    char *o, *ocopy, *dq, *dk, *dv;
+    const char *q, *k, *v, *doo, *att, *att_low;
+    char *o, *ocopy, *olow, *dq, *dk, *dv;
     float *lse, *delta, *part, *part_ml;
     const int *q_len, *k_len;
     long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, g_sb, g_ss, g_sh;   // strides in elements
@@ -276,6 +276,17 @@ __device__ __forceinline__ f32x4 load4(const char* p) {
         const T4 v = *reinterpret_cast<const T4*>(p);
         return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
     }
+}
+
+// one piece of a result row: o without the residual (16-bit types: and what its rounding leaves, so that the backward's delta is
+// not that of a rounded o — dq's error is then 1.4 times its own rounding's, not 1.53), and o
+template <typename T>
+__device__ __forceinline__ void store_o(const Args& a, long at, const char* residual, f32x4 o) {
+    if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
+    if (!std::is_same<T, float>::value && a.olow)
+        store4<T>(a.olow + at, o[0] - (float)(T)o[0], o[1] - (float)(T)o[1], o[2] - (float)(T)o[2], o[3] - (float)(T)o[3]);
+    if (residual) o += load4<T>(residual);
+    store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
 }
 
 // ---- tiles of ROWS rows through registers into LDS: requested while the previous tile is used -----------------------
@@ -564,9 +575,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
             if (row_ok && l != 0.f)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[j] = acc[d][4 * q4 + j] * inv;
-            if (a.ocopy) store4<T>(a.ocopy + orow + at, o[0], o[1], o[2], o[3]);
-            if (a.residual && row_ok) o += load4<T>(qrow + at);
-            store4<T>(a.o + orow + at, o[0], o[1], o[2], o[3]);
+            store_o<T>(a, orow + at, a.residual && row_ok ? qrow + at : nullptr, o);
         }
 }
 
@@ -759,10 +768,8 @@ __global__ __launch_bounds__(256) void fwd_rows_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = ok ? o[e] * inv : 0.f;
         const long at = ((((long)b * a.Sq + me.pos) * a.H + kh * a.G + me.g) * D + d4 * 4) * es;
-        if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
-        if (a.residual && me.ok)
-            o += load4<T>(a.q + (b * a.q_sb + me.pos * a.q_ss + (kh * a.G + me.g) * a.q_sh + d4 * 4) * es);
-        store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
+        store_o<T>(a, at, a.residual && me.ok ? a.q + (b * a.q_sb + me.pos * a.q_ss + (kh * a.G + me.g) * a.q_sh + d4 * 4) * es : nullptr,
+                   o);
     }
 }
 
@@ -822,9 +829,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = ok ? o[j] * inv : 0.f;
     const long es = sizeof(T), at = ((((long)b * a.Sq + pos) * a.H + head) * D + d4 * 4) * es;
-    if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
-    if (a.residual && pos < ql) o += load4<T>(a.q + (b * a.q_sb + pos * a.q_ss + head * a.q_sh + d4 * 4) * es);
-    store4<T>(a.o + at, o[0], o[1], o[2], o[3]);
+    store_o<T>(a, at, a.residual && pos < ql ? a.q + (b * a.q_sb + pos * a.q_ss + head * a.q_sh + d4 * 4) * es : nullptr, o);
 }
 
 // sum over the splits of the 4 values at `e` of n4, shared out over SG groups of 256 / SG threads; true in the group that
@@ -883,6 +888,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
     float dl, lse = INFINITY;
     {
         dl = dot_rows<T, D>(grow, a.att + orow, row_ok);
+        if (a.att_low) dl += dot_rows<T, D>(grow, a.att_low + orow, row_ok);
         if (row_ok) lse = a.lse[hrow];
         if (h == 0 && r < a.R && pl.split == 0) a.delta[hrow] = dl;
     }
@@ -1315,7 +1321,8 @@ static Args args_of(const cmvae_set_attn& d) {
     Args a = {};
     a.q = (const char*)d.q; a.k = (const char*)d.k; a.v = (const char*)d.v;
     a.doo = (const char*)d.dO;
-    a.o = (char*)d.o; a.ocopy = (char*)d.attn;
+    a.o = (char*)d.o; a.ocopy = (char*)d.attn; a.olow = (char*)d.attn_low;
+    a.att_low = (const char*)d.attn_low;
     a.att = (const char*)(d.residual ? d.attn : d.o);
     a.dq = (char*)d.dq; a.dk = (char*)d.dk; a.dv = (char*)d.dv;
     a.lse = d.lse; a.delta = d.delta;
@@ -1361,7 +1368,7 @@ extern "C" int cmvae_set_attention_fwd(const cmvae_set_attn* d, void* workspace,
     if (int e = sa::check_desc("cmvae_set_attention_fwd", d)) return e;
     CMVAE_REQUIRE(d->q && d->o && (d->Sk == 0 || (d->k && d->v)), "cmvae_set_attention_fwd: NULL tensor");
     CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype) && sa::aligned(d->k, d->k_stride, d->dtype) &&
-                      sa::aligned(d->v, d->v_stride, d->dtype) && ((uintptr_t)d->o & 15) == 0 && ((uintptr_t)d->attn & 15) == 0,
+                      sa::aligned(d->v, d->v_stride, d->dtype) && (((uintptr_t)d->o | (uintptr_t)d->attn | (uintptr_t)d->attn_low) & 15) == 0,
                   "cmvae_set_attention_fwd: rows must start at multiples of 16 bytes and lie under 2^22 elements apart");
     const sa::Sizes z = sa::sizes_of(*d);
     CMVAE_REQUIRE(z.fwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.fwd),
@@ -1378,7 +1385,7 @@ extern "C" int cmvae_set_attention_bwd(const cmvae_set_attn* d, void* workspace,
                   "cmvae_set_attention_bwd: NULL tensor");
     CMVAE_REQUIRE(sa::aligned(d->q, d->q_stride, d->dtype) && sa::aligned(d->k, d->k_stride, d->dtype) &&
                       sa::aligned(d->v, d->v_stride, d->dtype) && sa::aligned(d->dO, d->dO_stride, d->dtype) &&
-                      (((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv | (uintptr_t)d->o | (uintptr_t)d->attn) & 15) == 0,
+                      (((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv | (uintptr_t)d->o | (uintptr_t)d->attn | (uintptr_t)d->attn_low) & 15) == 0,
                   "cmvae_set_attention_bwd: rows must start at multiples of 16 bytes and lie under 2^22 elements apart");
     const sa::Sizes z = sa::sizes_of(*d);
     CMVAE_REQUIRE(z.bwd == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bwd),

@@ -129,15 +129,17 @@ class SetAttention : public torch::autograd::Function<SetAttention> {
         const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0);
         const SetAttentionArgs a = {scale, causal, residual};
         const Tensor o = at::empty(q.sizes(), q.options());
-        Tensor attn = o, lse;
+        Tensor attn = o, low, lse;
         if (save) {
             lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
             if (residual) attn = at::empty(q.sizes(), q.options());
+            if (q.scalar_type() != at::kFloat) low = at::empty(q.sizes(), q.options());
         }
         if (o.numel()) {
             cmvae_set_attn d = describe(q, k, v, a, ptr(q_len), ptr(k_len));
             d.o = o.data_ptr();
             d.attn = save && residual ? attn.data_ptr() : nullptr;
+            d.attn_low = ptr(low);
             d.lse = (float*)ptr(lse);
             const size_t n = lib.sa_ws(&d, 0);
             const Tensor ws = workspace(n, q);
@@ -147,7 +149,7 @@ class SetAttention : public torch::autograd::Function<SetAttention> {
             ctx->saved_data["scale"] = scale;
             ctx->saved_data["causal"] = causal;
             ctx->saved_data["residual"] = residual;
-            ctx->save_for_backward({q, k, v, attn, lse, given(q_len) ? *q_len : Tensor(), given(k_len) ? *k_len : Tensor()});
+            ctx->save_for_backward({q, k, v, attn, lse, given(q_len) ? *q_len : Tensor(), given(k_len) ? *k_len : Tensor(), low});
         }
         return o;
     }
@@ -173,6 +175,7 @@ class SetAttention : public torch::autograd::Function<SetAttention> {
                 d.dO = go.data_ptr();
                 strides3(d.dO_stride, go);
                 d.o = d.attn = attn.data_ptr();
+                d.attn_low = ptr(s[7]);
                 d.lse = (float*)lse.data_ptr(); d.delta = (float*)delta.data_ptr();
                 d.dq = dq.data_ptr(); d.dk = dk.data_ptr(); d.dv = dv.data_ptr();
                 const size_t n = lib.sa_ws(&d, 1);

@@ -298,8 +298,9 @@ int cmvae_attention_qkv_bwd(const float* QKV, const float* lse, const float* dO,
  * at multiples of 16 bytes and lie under 2^22 elements apart); D 64 or 128, H a multiple of Hkv (query head h reads key head h / (H / Hkv)).  o, attn, dq
  * [B,Sq,H,D] and dk, dv [B,Sk,Hkv,D] are dense.  q_len, k_len: int32 [B] or NULL (all rows), clamped to the tensors.
  * Values of rows behind a length are not read.  lse, delta: fp32 [B,H,Sq].  Forward: lse may be NULL; attn, if not NULL,
- * receives o without the residual.  Backward: reads o (residual: attn) and lse of the forward, writes delta (scratch),
- * dq, dk, dv; gradients of rows behind a length are zeros.                                                          */
+ * receives o without the residual, and attn_low (16-bit types, not NULL) what its rounding leaves.  Backward: reads o
+ * (residual: attn), attn_low if not NULL, and lse of the forward, writes delta (scratch), dq, dk, dv; gradients of rows
+ * behind a length are zeros.                                                          */
 #define CMVAE_F32 0
 #define CMVAE_BF16 1
 #define CMVAE_F16 2
@@ -309,7 +310,7 @@ typedef struct cmvae_set_attn {
     const void *q, *k, *v, *dO;
     int64_t q_stride[3], k_stride[3], v_stride[3], dO_stride[3];
     const int32_t *q_len, *k_len;
-    void *o, *attn;
+    void *o, *attn, *attn_low;
     float *lse, *delta;
     void *dq, *dk, *dv;
 } cmvae_set_attn;
