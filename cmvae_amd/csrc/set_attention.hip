@@ -299,8 +299,9 @@ struct Stage {
     static constexpr int N = ROWS * CPR / THREADS, STEP = THREADS / CPR;
     static_assert(ROWS * CPR % THREADS == 0 && THREADS % CPR == 0, "whole pieces per thread");
     u32x4 x[N];
+    __device__ __forceinline__ static int tid() { return (int)threadIdx.x % THREADS; }
     __device__ __forceinline__ static unsigned offset(long stride) {
-        return (unsigned)((int)threadIdx.x / CPR * (int)stride + (int)threadIdx.x % CPR * 16);
+        return (unsigned)(tid() / CPR * (int)stride + tid() % CPR * 16);
     }
     // `left` rows from `base` on, the others are zeros
     __device__ __forceinline__ void load(const char* base, long stride, unsigned off, int left) {
@@ -311,7 +312,7 @@ struct Stage {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 x[i] = u32x4{0, 0, 0, 0};
-                if (i * STEP + (int)threadIdx.x / CPR < left) x[i] = *reinterpret_cast<const u32x4*>(base + i * STEP * stride + off);
+                if (i * STEP + tid() / CPR < left) x[i] = *reinterpret_cast<const u32x4*>(base + i * STEP * stride + off);
             }
         }
     }
@@ -319,18 +320,18 @@ struct Stage {
     __device__ __forceinline__ void load_across(const char* base, long ss, long sh, int g, int pos, int left, int ql) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int j = i * STEP + (int)threadIdx.x / CPR;
+            const int j = i * STEP + tid() / CPR;
             x[i] = u32x4{0, 0, 0, 0};
             if (j < left) {
                 const int q = (pos + j) / ql;
-                x[i] = *reinterpret_cast<const u32x4*>(base + (pos + j - q * ql) * ss + (g + q) * sh + (int)threadIdx.x % CPR * 16);
+                x[i] = *reinterpret_cast<const u32x4*>(base + (pos + j - q * ql) * ss + (g + q) * sh + tid() % CPR * 16);
             }
         }
     }
     __device__ __forceinline__ void put(char* tile, const Sel& sel) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = i * THREADS + threadIdx.x;
+            const int id = i * THREADS + tid();
             char* at = tile + (id / CPR) * pitch<D>() + (id % CPR) * (Elem<T>::P == 3 ? 8 : 16);
             if constexpr (Elem<T>::P == 3) {
                 const f32x4 v = __builtin_bit_cast(f32x4, x[i]);
@@ -447,18 +448,56 @@ __device__ __forceinline__ void span(int ql, int r0, int r1, int& lo, int& hi) {
     hi = g0 == g1 ? r1 - 1 - g0 * ql : ql - 1;
 }
 
+// Waves of a workgroup: NW waves of 32 own rows that share the tiles they walk (two buffers, one barrier per tile) — or, where
+// there are few rows, WS waves that share the same 32 own rows and walk every WS-th tile, each in a buffer of its own without
+// a barrier, and meet at the end: one launch where pieces of the walk would need a second one to join them.
+template <typename T, int D>
+constexpr int walkers() { return sizeof(T) * D > 256 ? 2 : 4; }      // fp32 heads of 128: 52 KB of planes per wave
+
+// orders a wave's own LDS accesses across its lanes (the hardware runs them in order; this keeps the compiler to it)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// wave w > 0 hands an accumulator to wave 0 (the buffers are free: all waves are through)
+template <int WS, int N>
+__device__ __forceinline__ void hand_over(char* smem, int w, const f32x16 (&acc)[N]) {
+    __syncthreads();
+    if (w > 0)
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                reinterpret_cast<f32x4*>(smem)[(((w - 1) * N + d) * 4 + q) * 64 + (threadIdx.x & 63)] =
+                    f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
+    __syncthreads();
+}
+template <int N>
+__device__ __forceinline__ void take_over(const char* smem, int w, float f, f32x16 (&acc)[N]) {
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 x = reinterpret_cast<const f32x4*>(smem)[(((w - 1) * N + d) * 4 + q) * 64 + (threadIdx.x & 63)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[d][4 * q + j] = fmaf(x[j], f, acc[d][4 * q + j]);
+        }
+}
+
 // ------------------------------------------------------------------------------------------------ forward
-// NW waves of 32 rows; keys in tiles of KT through LDS, two buffers.  Running maximum m (log2 units) and sum l per row.
+// Keys in tiles of KT through LDS.  Running maximum m (log2 units) and sum l per row.
 // nsplit > 1: a workgroup covers split_tiles tiles and leaves (acc, m, l) for the joining kernel.
-template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
+template <typename T, int D, int NW, int KT, int WS>
+__global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = Elem<T>::P * KT * pitch<D>();
     const Place pl = place<NW * 32, false>(a);
     const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
-    const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
+    const int r0 = pl.tile * NW * 32, r = r0 + (WS > 1 ? 0 : w) * 32 + (lane & 31);
     const Row me = row_of(a, ql, r);
     const int g = me.g, pos = me.pos;
     const bool row_ok = me.ok;
@@ -494,16 +533,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
         ks.load(kb + (long)t * KT * ksb, ksb, ko, kl - t * KT);
         vs.load(vb + (long)t * KT * vsb, vsb, vo, kl - t * KT);
     };
-    if (t0 < t1) {
-        request(t0);
-        ks.put(smem, sel);
-        vs.put(smem + TB, sel);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const char* kt = smem + ((t - t0) & 1) * 2 * TB;
-        const char* vt = kt + TB;
-        if (t + 1 < t1) request(t + 1);
+    auto use = [&](int t, const char* kt, const char* vt) {
         f32x16 s[KT / 32];
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) s[u] = mul_rows<T, D, KT>(kt, u * 32, qf, zero16());
@@ -538,14 +568,60 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void fwd_ker
         for (int d = 0; d < D / 32; ++d) acc[d] *= al;
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) mul_cols<T, D, KT>(vt, u * 32, s[u], sel, acc);
-        if (t + 1 < t1) {
-            char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
-            ks.put(nx, sel);
-            vs.put(nx + TB, sel);
+    };
+    if constexpr (WS > 1) {
+        char* my = smem + w * 2 * TB;
+        int t = t0 + w;
+        if (t < t1) request(t);
+        for (; t < t1; t += WS) {
+            ks.put(my, sel);
+            vs.put(my + TB, sel);
+            wave_sync();
+            if (t + WS < t1) request(t + WS);
+            use(t, my, my + TB);
+            wave_sync();
+        }
+    } else {
+        if (t0 < t1) {
+            request(t0);
+            ks.put(smem, sel);
+            vs.put(smem + TB, sel);
         }
         __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            const char* kt = smem + ((t - t0) & 1) * 2 * TB;
+            if (t + 1 < t1) request(t + 1);
+            use(t, kt, kt + TB);
+            if (t + 1 < t1) {
+                char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
+                ks.put(nx, sel);
+                vs.put(nx + TB, sel);
+            }
+            __syncthreads();
+        }
     }
     l += other_half(l);
+    if constexpr (WS > 1) {
+        __shared__ float sm[WS][64], sl[WS][64];
+        sm[w][lane] = m;
+        sl[w][lane] = l;
+        hand_over<WS>(smem, w, acc);
+        if (w > 0) return;
+        float mx = m;
+#pragma unroll
+        for (int i = 1; i < WS; ++i) mx = fmaxf(mx, sm[i][lane]);
+        const float mu = mx == -INFINITY ? 0.f : mx, f0 = exp2_raw(m - mu);
+        l *= f0;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= f0;
+#pragma unroll
+        for (int i = 1; i < WS; ++i) {
+            const float fi = exp2_raw(sm[i][lane] - mu);
+            l = fmaf(sl[i][lane], fi, l);
+            take_over(smem, i, fi, acc);
+        }
+        m = mx;
+    }
     if (r >= a.R) return;
     const long hrow = ((long)pl.b * a.H + pl.kh * a.G + g) * a.Sq + pos;
     if (a.nsplit > 1) {
@@ -851,15 +927,15 @@ __device__ __forceinline__ bool join_sum(const Args& a, const float* part, long 
 
 // ------------------------------------------------------------------------------------------------ backward, query side
 // The forward's shape; delta_i from the saved o, kept for the key side.
-template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
+template <typename T, int D, int NW, int KT, int WS>
+__global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = Elem<T>::P * KT * pitch<D>();
     const Place pl = place<NW * 32, false>(a);
     const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, rv = a.G * ql;
-    const int r0 = pl.tile * NW * 32, r = r0 + w * 32 + (lane & 31);
+    const int r0 = pl.tile * NW * 32, r = r0 + (WS > 1 ? 0 : w) * 32 + (lane & 31);
     const Row me = row_of(a, ql, r);
     const int g = me.g, pos = me.pos;
     const bool row_ok = me.ok;
@@ -890,7 +966,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
         dl = dot_rows<T, D>(grow, a.att + orow, row_ok);
         if (a.att_low) dl += dot_rows<T, D>(grow, a.att_low + orow, row_ok);
         if (row_ok) lse = a.lse[hrow];
-        if (h == 0 && r < a.R && pl.split == 0) a.delta[hrow] = dl;
+        if (h == 0 && r < a.R && pl.split == 0 && (WS == 1 || w == 0)) a.delta[hrow] = dl;
     }
     f32x16 acc[D / 32];
 #pragma unroll
@@ -905,16 +981,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
         ks.load(kb + (long)t * KT * ksb, ksb, ko, kl - t * KT);
         vs.load(vb + (long)t * KT * vsb, vsb, vo, kl - t * KT);
     };
-    if (t0 < t1) {
-        request(t0);
-        ks.put(smem, sel);
-        vs.put(smem + TB, sel);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const char* kt = smem + ((t - t0) & 1) * 2 * TB;
-        const char* vt = kt + TB;
-        if (t + 1 < t1) request(t + 1);
+    auto use = [&](int t, const char* kt, const char* vt) {
         const int k0 = t * KT;
         const bool edge = k0 + KT > kl || (a.causal && k0 + KT > lo + off + 1);
 #pragma unroll
@@ -930,12 +997,41 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 256 ? 2 : 1) void dq_kern
             }
             mul_cols<T, D, KT>(kt, u * 32, s, sel, acc);
         }
-        if (t + 1 < t1) {
-            char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
-            ks.put(nx, sel);
-            vs.put(nx + TB, sel);
+    };
+    if constexpr (WS > 1) {
+        char* my = smem + w * 2 * TB;
+        int t = t0 + w;
+        if (t < t1) request(t);
+        for (; t < t1; t += WS) {
+            ks.put(my, sel);
+            vs.put(my + TB, sel);
+            wave_sync();
+            if (t + WS < t1) request(t + WS);
+            use(t, my, my + TB);
+            wave_sync();
+        }
+        hand_over<WS>(smem, w, acc);
+        if (w > 0) return;
+#pragma unroll
+        for (int i = 1; i < WS; ++i) take_over(smem, i, 1.f, acc);
+    } else {
+        if (t0 < t1) {
+            request(t0);
+            ks.put(smem, sel);
+            vs.put(smem + TB, sel);
         }
         __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            const char* kt = smem + ((t - t0) & 1) * 2 * TB;
+            if (t + 1 < t1) request(t + 1);
+            use(t, kt, kt + TB);
+            if (t + 1 < t1) {
+                char* nx = smem + ((t + 1 - t0) & 1) * 2 * TB;
+                ks.put(nx, sel);
+                vs.put(nx + TB, sel);
+            }
+            __syncthreads();
+        }
     }
     if (r >= a.R) return;
     float* po = a.nsplit > 1 ? a.part + ((long)pl.split * a.B * a.Hkv * a.R + hrow) * D : nullptr;
@@ -975,16 +1071,16 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward, key side
-// NW waves of 32 keys; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
-template <typename T, int D, int NW, int RT>
-__global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof(T) * D == 256 && sizeof(T) == 4) ? 2 : 1) void dkv_kernel(Args a) {
+// 32 keys per wave; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
+template <typename T, int D, int NW, int RT, int WS>
+__global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (sizeof(T) == 4 && D == 64)) ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int TB = Elem<T>::P * RT * pitch<D>(), BUF = 2 * TB + RT * 8;
     const Place pl = place<NW * 32, true>(a);
     const Sel sel = make_sel();
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const int ql = pl.ql, kl = pl.kl, off = kl - ql, rv = a.G * ql;
-    const int key0 = pl.tile * NW * 32, key = key0 + w * 32 + (lane & 31);
+    const int key0 = pl.tile * NW * 32, key = key0 + (WS > 1 ? 0 : w) * 32 + (lane & 31);
     const bool key_ok = key < kl;
     const long es = sizeof(T);
     const Frag<T, D> kf = load_frag<T, D>(a.k + (pl.b * a.k_sb + key * a.k_ss + pl.kh * a.k_sh) * es, key_ok, sel);
@@ -1038,8 +1134,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
             qs.load_across(qb, qss, qsh, x.g, x.pos, left, ql);
             gs.load_across(gb, gss, gsh, x.g, x.pos, left, ql);
         }
-        if (threadIdx.x < RT) {
-            const int j = threadIdx.x;
+        if (St::tid() < RT) {
+            const int j = St::tid();
             st_lse = INFINITY;
             st_dl = 0.f;
             if (j < left) {
@@ -1053,9 +1149,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
     auto put = [&](char* buf) {
         qs.put(buf, sel);
         gs.put(buf + TB, sel);
-        if (threadIdx.x < RT) {
-            reinterpret_cast<float*>(buf + 2 * TB)[threadIdx.x] = st_lse;
-            reinterpret_cast<float*>(buf + 2 * TB)[RT + threadIdx.x] = st_dl;
+        if (St::tid() < RT) {
+            reinterpret_cast<float*>(buf + 2 * TB)[St::tid()] = st_lse;
+            reinterpret_cast<float*>(buf + 2 * TB)[RT + St::tid()] = st_dl;
         }
     };
     At x = {t, 0, 0};
@@ -1064,16 +1160,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
         x.pos = t * RT - x.g * ql;
         x = next(x);
     }
-    if (x.t < t1) {
-        request(x);
-        put(smem);
-    }
-    __syncthreads();
-    int cur = 0;
-    while (x.t < t1) {
-        const char* buf = smem + cur * BUF;
-        const At xn = next(step(x));
-        if (xn.t < t1) request(xn);
+    auto use = [&](const At& x, const char* buf) {
         const bool across = x.pos + RT > ql;
         const bool edge = a.causal && (across ? 0 : x.pos) + off < key0 + NW * 32 - 1;
 #pragma unroll
@@ -1104,10 +1191,48 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) * D <= 128 || (NW == 4 && sizeof
             }
             mul_cols<T, D, RT>(buf, u * 32, s, sel, dk);
         }
-        if (xn.t < t1) put(smem + (cur ^ 1) * BUF);
+    };
+    if constexpr (WS > 1) {
+        char* my = smem + w * BUF;
+        auto jump = [&](At x, int n) {                            // n tiles with a valid pair on
+            for (; n > 0 && x.t < t1; --n) x = next(step(x));
+            return x;
+        };
+        x = jump(x, w);
+        if (x.t < t1) request(x);
+        while (x.t < t1) {
+            put(my);
+            wave_sync();
+            const At xn = jump(x, WS);
+            if (xn.t < t1) request(xn);
+            use(x, my);
+            wave_sync();
+            x = xn;
+        }
+        hand_over<WS>(smem, w, dk);
+        if (w == 0)
+#pragma unroll
+            for (int i = 1; i < WS; ++i) take_over(smem, i, 1.f, dk);
+        hand_over<WS>(smem, w, dv);
+        if (w > 0) return;
+#pragma unroll
+        for (int i = 1; i < WS; ++i) take_over(smem, i, 1.f, dv);
+    } else {
+        if (x.t < t1) {
+            request(x);
+            put(smem);
+        }
         __syncthreads();
-        cur ^= 1;
-        x = xn;
+        int cur = 0;
+        while (x.t < t1) {
+            const At xn = next(step(x));
+            if (xn.t < t1) request(xn);
+            use(x, smem + cur * BUF);
+            if (xn.t < t1) put(smem + (cur ^ 1) * BUF);
+            __syncthreads();
+            cur ^= 1;
+            x = xn;
+        }
     }
     if (key >= a.Sk) return;
     const long krow = ((long)pl.b * a.Sk + key) * a.Hkv + pl.kh;
@@ -1158,10 +1283,11 @@ struct Plan {
     size_t lds;
 };
 
-// `rows` own rows in tiles of 32 per wave, `len` rows to walk; `occ` workgroups of four waves fit on a compute unit.  Four
-// waves share what they walk; where that leaves most of the card idle, one wave per workgroup.  The walk is cut into pieces,
-// which a second launch joins, until there is work for every wave slot — twice that for the causal order at one
-// workgroup per unit (two are dealt in pairs, see place()), and half again as much where lengths will leave some without work.
+// `rows` own rows in tiles of 32, `len` rows to walk; `occ` workgroups of four waves fit on a compute unit.  Four tiles of
+// own rows per workgroup share what they walk; where that leaves compute units without work, one tile per workgroup, whose
+// waves share out the walk.  The walk is cut into pieces, which a second launch joins, until there is a workgroup for every
+// slot — twice that for the causal order at one workgroup per unit (two are dealt in pairs, see place()), and half again as
+// much where lengths will leave some without work.
 static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats, int occ, bool causal, bool ragged) {
     Plan p;
     p.piece = 0;
@@ -1171,17 +1297,18 @@ static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats,
     p.tile = p.nw == 4 && esize == 2 ? 64 : 32;
     p.ntiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
     p.nsplit = 1;
-    const int tiles = (len + p.tile - 1) / p.tile;
+    const int tiles = (len + p.tile - 1) / p.tile, ws = esize * D > 256 ? 2 : 4;
     const long wg = nbh * p.ntiles;
-    long want = p.nw == 4 ? cus * occ : 4 * cus;
+    long want = p.nw == 4 ? cus * occ : cus;
     if (p.nw == 4) want = causal && occ == 1 ? 2 * want : ragged ? want + want / 2 : want;
-    const int least = p.nw == 4 ? 4 : 2;          // tiles per piece
+    const int least = p.nw == 4 ? 4 : 2 * ws;      // tiles per piece
     if (wg > 0 && wg < want && tiles >= 2 * least) {
         long ns = (want + wg - 1) / wg;
         if (ns > tiles / least) ns = tiles / least;
         p.nsplit = (int)(ns > 64 ? 64 : ns);
     }
-    p.lds = 2 * ((size_t)2 * (esize == 4 ? 3 : 1) * p.tile * (D * 2 + 16) + (stats ? p.tile * 8 : 0));
+    const size_t buf = (size_t)2 * (esize == 4 ? 3 : 1) * p.tile * (D * 2 + 16) + (stats ? p.tile * 8 : 0);
+    p.lds = (p.nw == 4 ? 2 : ws) * buf;
     return p;
 }
 
@@ -1250,7 +1377,7 @@ static int join_groups(int nsplit, long n4, int most) {
 
 template <typename T, int D>
 static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
-    constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
+    constexpr int T4 = sizeof(T) == 2 ? 64 : 32, WS = walkers<T, D>();
     const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R;
     use(a, z.f);
     a.part = ws;
@@ -1261,8 +1388,8 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
             : a.R == 2 ? launch(fwd_rows_kernel<T, D, 2>, blocks, 256, 0, a, stream, what)
             : a.R <= 4 ? launch(fwd_rows_kernel<T, D, 4>, blocks, 256, 0, a, stream, what)
             : a.R <= 8 ? launch(fwd_rows_kernel<T, D, 8>, blocks, 256, 0, a, stream, what)
-            : z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
-                        : launch(fwd_kernel<T, D, 1, 32>, blocks, 64, z.f.lds, a, stream, "set_attention fwd_kernel");
+            : z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4, 1>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
+                        : launch(fwd_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.f.lds, a, stream, "set_attention fwd_kernel");
     if (e || a.nsplit == 1) return e;
     a.sg = join_groups(a.nsplit, rows * (D / 4), 256 / (D / 4));
     return launch(fwd_join_kernel<T, D>, (rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
@@ -1270,13 +1397,13 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
 
 template <typename T, int D>
 static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
-    constexpr int T4 = sizeof(T) == 2 ? 64 : 32;
+    constexpr int T4 = sizeof(T) == 2 ? 64 : 32, WS = walkers<T, D>();
     const long nbh = (long)a.B * a.Hkv, rows = nbh * a.R, keys = nbh * a.Sk;
     a.part = ws;
     use(a, z.q);
     long blocks = nbh * a.ntiles * a.nsplit;
-    int e = z.q.nw == 4 ? launch(dq_kernel<T, D, 4, T4>, blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
-                        : launch(dq_kernel<T, D, 1, 32>, blocks, 64, z.q.lds, a, stream, "set_attention dq_kernel");
+    int e = z.q.nw == 4 ? launch(dq_kernel<T, D, 4, T4, 1>, blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
+                        : launch(dq_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.q.lds, a, stream, "set_attention dq_kernel");
     if (e) return e;
     if (a.nsplit > 1) {
         a.sg = join_groups(a.nsplit, rows * (D / 4), 16);
@@ -1285,8 +1412,8 @@ static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
     }
     use(a, z.k);
     blocks = nbh * a.ntiles * a.nsplit;
-    e = z.k.nw == 4 ? launch(dkv_kernel<T, D, 4, T4>, blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
-                    : launch(dkv_kernel<T, D, 1, 32>, blocks, 64, z.k.lds, a, stream, "set_attention dkv_kernel");
+    e = z.k.nw == 4 ? launch(dkv_kernel<T, D, 4, T4, 1>, blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
+                    : launch(dkv_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.k.lds, a, stream, "set_attention dkv_kernel");
     if (e || a.nsplit == 1) return e;
     const long n4 = keys * D / 4;
     a.sg = join_groups(a.nsplit, n4, 16);
