@@ -1,6 +1,7 @@
 // Shared host/device helpers for libcmvae_hip.so (gfx950 only).
 #pragma once
 #include <hip/hip_runtime.h>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdint>
@@ -53,6 +54,26 @@ inline int compute_units() {
         return n;
     }();
     return cus;
+}
+
+// Launch of a kernel that takes its arguments as one struct.  More than 64 KB of dynamic LDS needs the opt-in, once per
+// kernel and device (asked for at every launch it would be 1-2 us of the host's).
+template <auto KERNEL, typename ARGS>
+inline int launch_kernel(long blocks, int threads, size_t lds, const ARGS& args, void* stream, const char* what) {
+    if (blocks == 0) return 0;
+    if (lds > 64 * 1024) {
+        static std::atomic<unsigned long long> asked{0};
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (!(asked.load(std::memory_order_relaxed) & bit)) {
+            const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, 152 * 1024);
+            if (e != hipSuccess) return set_error("%s: %s", what, hipGetErrorString(e));
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, args);
+    return check_launch(what);
 }
 
 inline size_t align_up(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }

@@ -601,32 +601,22 @@ static size_t ws_bytes(const cmvae_group_norm& d, const Plan& p, bool backward) 
     return nc * sizeof(float2) + 256 + (size_t)d.N * d.G * sizeof(float2);
 }
 
-template <typename K>
-static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a, void* stream, const char* what) {
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return set_error("%s: %s", what, hipGetErrorString(e));
-    }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, a);
-    return check_launch(what);
-}
-
 template <typename T, int V>
 static int run_fwd(Args a, const Plan& p, void* stream) {
     if (p.threads) {
         const size_t lds = (size_t)p.threads * V * sizeof(double2) + a.G * sizeof(float4);
         const char* what = "group_norm fwd_resident_kernel";
         switch (p.threads) {
-            case 64: return launch(fwd_resident_kernel<T, V, 64, 2>, a.N, 64, lds, a, stream, what);
-            case 256: return launch(fwd_resident_kernel<T, V, 256, 2>, a.N, 256, lds, a, stream, what);
-            case 512: return launch(fwd_resident_kernel<T, V, 512, 8>, a.N, 512, lds, a, stream, what);
-            default: return launch(fwd_resident_kernel<T, V, 1024, 16>, a.N, 1024, lds, a, stream, what);
+            case 64: return launch_kernel<fwd_resident_kernel<T, V, 64, 2>>(a.N, 64, lds, a, stream, what);
+            case 256: return launch_kernel<fwd_resident_kernel<T, V, 256, 2>>(a.N, 256, lds, a, stream, what);
+            case 512: return launch_kernel<fwd_resident_kernel<T, V, 512, 8>>(a.N, 512, lds, a, stream, what);
+            default: return launch_kernel<fwd_resident_kernel<T, V, 1024, 16>>(a.N, 1024, lds, a, stream, what);
         }
     }
     const long blocks = (long)a.N * a.pc * a.cc;
-    if (int e = launch(fwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_sums_kernel")) return e;
-    if (int e = launch(fwd_finish_kernel, (long)a.N * a.G, 256, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
-    return launch(fwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm fwd_apply_kernel");
+    if (int e = launch_kernel<fwd_sums_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm fwd_sums_kernel")) return e;
+    if (int e = launch_kernel<fwd_finish_kernel>((long)a.N * a.G, 256, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
+    return launch_kernel<fwd_apply_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm fwd_apply_kernel");
 }
 
 template <typename T, int V>
@@ -636,16 +626,16 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
         const size_t lds = (size_t)p.threads * V * sizeof(float2) + a.G * (sizeof(float4) + sizeof(float2));
         const char* what = "group_norm bwd_resident_kernel";
         switch (p.threads) {
-            case 64: e = launch(bwd_resident_kernel<T, V, 64, 2>, a.N, 64, lds, a, stream, what); break;
-            case 256: e = launch(bwd_resident_kernel<T, V, 256, 2>, a.N, 256, lds, a, stream, what); break;
-            case 512: e = launch(bwd_resident_kernel<T, V, 512, 8>, a.N, 512, lds, a, stream, what); break;
-            default: e = launch(bwd_resident_kernel<T, V, 1024, 8>, a.N, 1024, lds, a, stream, what);
+            case 64: e = launch_kernel<bwd_resident_kernel<T, V, 64, 2>>(a.N, 64, lds, a, stream, what); break;
+            case 256: e = launch_kernel<bwd_resident_kernel<T, V, 256, 2>>(a.N, 256, lds, a, stream, what); break;
+            case 512: e = launch_kernel<bwd_resident_kernel<T, V, 512, 8>>(a.N, 512, lds, a, stream, what); break;
+            default: e = launch_kernel<bwd_resident_kernel<T, V, 1024, 8>>(a.N, 1024, lds, a, stream, what);
         }
     } else {
         const long blocks = (long)a.N * a.pc * a.cc;
-        if ((e = launch(bwd_sums_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_sums_kernel"))) return e;
-        if ((e = launch(bwd_finish_kernel, (long)a.N * a.G, 256, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
-        e = launch(bwd_apply_kernel<T, V>, blocks, 256, 0, a, stream, "group_norm bwd_apply_kernel");
+        if ((e = launch_kernel<bwd_sums_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm bwd_sums_kernel"))) return e;
+        if ((e = launch_kernel<bwd_finish_kernel>((long)a.N * a.G, 256, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
+        e = launch_kernel<bwd_apply_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm bwd_apply_kernel");
     }
     if (e || (!a.dw && !a.db)) return e;
     hipLaunchKernelGGL(param_grad_kernel, dim3((a.C + 3) / 4), dim3(256), 0, (hipStream_t)stream, a, (long)a.N * a.pc);

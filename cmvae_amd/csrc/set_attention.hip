@@ -1350,17 +1350,6 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     return z;
 }
 
-template <typename K>
-static int launch(K kernel, long blocks, int threads, size_t lds, const Args& a, void* stream, const char* what) {
-    if (blocks == 0) return 0;                    // no keys: there is no key side
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return set_error("%s: %s", what, hipGetErrorString(e));
-    }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, a);
-    return check_launch(what);
-}
-
 static void use(Args& a, const Plan& p) {
     a.ntiles = p.ntiles;
     a.nsplit = p.nsplit;
@@ -1384,15 +1373,15 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
     a.part_ml = ws + (size_t)a.nsplit * rows * D;
     const long blocks = nbh * a.ntiles * a.nsplit;
     const char* what = "set_attention fwd_rows_kernel";
-    int e = a.R == 1 ? launch(fwd_rows_kernel<T, D, 1>, blocks, 256, 0, a, stream, what)
-            : a.R == 2 ? launch(fwd_rows_kernel<T, D, 2>, blocks, 256, 0, a, stream, what)
-            : a.R <= 4 ? launch(fwd_rows_kernel<T, D, 4>, blocks, 256, 0, a, stream, what)
-            : a.R <= 8 ? launch(fwd_rows_kernel<T, D, 8>, blocks, 256, 0, a, stream, what)
-            : z.f.nw == 4 ? launch(fwd_kernel<T, D, 4, T4, 1>, blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
-                        : launch(fwd_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.f.lds, a, stream, "set_attention fwd_kernel");
+    int e = a.R == 1 ? launch_kernel<fwd_rows_kernel<T, D, 1>>(blocks, 256, 0, a, stream, what)
+            : a.R == 2 ? launch_kernel<fwd_rows_kernel<T, D, 2>>(blocks, 256, 0, a, stream, what)
+            : a.R <= 4 ? launch_kernel<fwd_rows_kernel<T, D, 4>>(blocks, 256, 0, a, stream, what)
+            : a.R <= 8 ? launch_kernel<fwd_rows_kernel<T, D, 8>>(blocks, 256, 0, a, stream, what)
+            : z.f.nw == 4 ? launch_kernel<fwd_kernel<T, D, 4, T4, 1>>(blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
+                        : launch_kernel<fwd_kernel<T, D, 1, 32, WS>>(blocks, WS * 64, z.f.lds, a, stream, "set_attention fwd_kernel");
     if (e || a.nsplit == 1) return e;
     a.sg = join_groups(a.nsplit, rows * (D / 4), 256 / (D / 4));
-    return launch(fwd_join_kernel<T, D>, (rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
+    return launch_kernel<fwd_join_kernel<T, D>>((rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
 }
 
 template <typename T, int D>
@@ -1402,22 +1391,22 @@ static int run_bwd(Args a, const Sizes& z, float* ws, void* stream) {
     a.part = ws;
     use(a, z.q);
     long blocks = nbh * a.ntiles * a.nsplit;
-    int e = z.q.nw == 4 ? launch(dq_kernel<T, D, 4, T4, 1>, blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
-                        : launch(dq_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.q.lds, a, stream, "set_attention dq_kernel");
+    int e = z.q.nw == 4 ? launch_kernel<dq_kernel<T, D, 4, T4, 1>>(blocks, 256, z.q.lds, a, stream, "set_attention dq_kernel")
+                        : launch_kernel<dq_kernel<T, D, 1, 32, WS>>(blocks, WS * 64, z.q.lds, a, stream, "set_attention dq_kernel");
     if (e) return e;
     if (a.nsplit > 1) {
         a.sg = join_groups(a.nsplit, rows * (D / 4), 16);
-        if ((e = launch(dq_join_kernel<T, D>, (rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dq_join_kernel")))
+        if ((e = launch_kernel<dq_join_kernel<T, D>>((rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dq_join_kernel")))
             return e;
     }
     use(a, z.k);
     blocks = nbh * a.ntiles * a.nsplit;
-    e = z.k.nw == 4 ? launch(dkv_kernel<T, D, 4, T4, 1>, blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
-                    : launch(dkv_kernel<T, D, 1, 32, WS>, blocks, WS * 64, z.k.lds, a, stream, "set_attention dkv_kernel");
+    e = z.k.nw == 4 ? launch_kernel<dkv_kernel<T, D, 4, T4, 1>>(blocks, 256, z.k.lds, a, stream, "set_attention dkv_kernel")
+                    : launch_kernel<dkv_kernel<T, D, 1, 32, WS>>(blocks, WS * 64, z.k.lds, a, stream, "set_attention dkv_kernel");
     if (e || a.nsplit == 1) return e;
     const long n4 = keys * D / 4;
     a.sg = join_groups(a.nsplit, n4, 16);
-    return launch(dkv_join_kernel<T, D>, (n4 * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dkv_join_kernel");
+    return launch_kernel<dkv_join_kernel<T, D>>((n4 * a.sg + 255) / 256, 256, 0, a, stream, "set_attention dkv_join_kernel");
 }
 
 static bool aligned(const void* p, const int64_t* s, int dtype) {
