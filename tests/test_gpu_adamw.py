@@ -299,3 +299,29 @@ def test_refusals(device):
         adamw_state_values(m, v, None)
     with pytest.raises(RuntimeError, match='AdamW'):
         AdamW([p], state_bits=16)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_more_values_than_32_bits_count(device, bits):
+    """A tensor of 2^31 + 300 values, with something in its last 1024 only, behind a small one: they become what a tensor of
+    those 1024 becomes, the others stay."""
+    from cmvae_amd.optim import adamw_step, state_size
+    n, tail = 2 ** 31 + 300, 300 + 256 * 3
+    small, gs, m, v, sc = make(device, [(tail,)], torch.bfloat16, bits, seed=5)
+    k = state_size(n) + 256
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device=device) for _ in range(2))
+    p[-tail:], g[-tail:] = small[0], gs[0]
+    M, V = (torch.zeros(k * x.element_size(), dtype=torch.uint8, device=device).view(x.dtype) for x in (m, v))
+    at = k - m.numel()
+    M[at:], V[at:] = m, v
+    S = None
+    if bits == 8:
+        S = torch.zeros(2, k // 256, device=device)
+        S[:, at // 256:] = sc
+    one = [torch.ones(2, dtype=torch.bfloat16, device=device) for _ in range(2)]
+    adamw_step([one[0], p], [one[1], g], M, V, S, step=7, **HYPER)
+    adamw_step(small, gs, m, v, sc, step=7, **HYPER)
+    assert torch.equal(p[-tail:], small[0]) and not p[:-tail].any()
+    assert torch.equal(M[at:].view(torch.uint8), m.view(torch.uint8)) and torch.equal(V[at:], v)
+    assert sc is None or torch.equal(S[:, at // 256:], sc)
+    assert not V[256:at].any()

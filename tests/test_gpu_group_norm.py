@@ -239,3 +239,31 @@ def test_refusals(device):
                      ((x[:, :, :0], 1), {})]:
         with pytest.raises(RuntimeError, match='group_norm_act'):
             group_norm_act(*args, **kw)
+
+
+@pytest.mark.parametrize('P', [40, 300])
+def test_offsets_beyond_32_bits(device, P):
+    """Pixels 2^23 elements apart: the 257th lies past 2^31 elements.  With 40 of them it is the second sample that does."""
+    apart, sample = 2 ** 23, 2 ** 31 if P == 40 else 64
+    x, w, b, dy = make(device, 2, (P,), 64, 'bf16')
+    buf = torch.empty(sample + P * apart, dtype=torch.bfloat16, device=device)
+    far = buf.as_strided((2, P, 64), (sample, apart, 1))
+    far.copy_(x)
+    want = run(x, w, b, dy, 8, act='silu')
+    assert all(torch.equal(s, t) for s, t in zip(want, run(far, w, b, dy, 8, act='silu')))
+
+
+def test_two_calls_at_once(device):
+    """Calls in flight on two streams use workspaces of their own."""
+    sets = [make(device, 2, (40, 40), 320, 'f32', seed=s) for s in (1, 2)]
+    want = [run(*s, 32, act='elu') for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(run(*s, 32, act='elu'))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for a, b in zip(want, got) for x, y in zip(a, b))

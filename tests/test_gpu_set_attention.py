@@ -276,3 +276,58 @@ def test_refusals(device):
     for args, kw in bad:
         with pytest.raises(RuntimeError, match='set_attention'):
             set_attention(*args, **kw)
+
+
+# more entries than one lane each, lists of 3, 6, 8 and 16 rows, tiles that span several short heads, pieces of long walks
+MORE = {
+    'seventy_entries': (70, 37, 90, 2, 1, 64, True, [37 - b % 38 for b in range(70)], [90 - (7 * b) % 91 for b in range(70)], True),
+    'seventy_entries_wide': (70, 140, 66, 8, 8, 64, False, None, [66 - b % 67 for b in range(70)], False),
+    'three_rows': (2, 1, 2500, 6, 2, 64, False, None, [2500, 7], True),
+    'six_rows': (3, 3, 777, 4, 2, 128, True, [3, 2, 0], [777, 1, 500], False),
+    'eight_rows': (2, 4, 1500, 4, 2, 64, True, None, [1500, 3], True),
+    'sixteen_rows': (2, 1, 5000, 32, 2, 128, True, None, [5000, 1234], False),
+    'short_heads': (2, 5, 300, 16, 2, 64, True, [5, 3], [300, 4], False),
+    'odd_group': (2, 75, 210, 9, 3, 128, True, [75, 31], [210, 31], True),
+    'all_masked': (2, 30, 40, 2, 2, 64, True, [0, 30], [40, 0], False),
+}
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('case', MORE)
+def test_more_shapes_against_float64(device, case, dtype):
+    B, Sq, Sk, H, Hkv, D, causal, ql, kl, residual = MORE[case]
+    q, k, v, do = make(device, B, Sq, Sk, H, Hkv, D, dtype, seed=4)
+    got = run(q, k, v, do, causal=causal, q_len=lens(ql, device), k_len=lens(kl, device), residual=residual)
+    want, tol = reference(q, k, v, do, 1 / math.sqrt(D), causal, ql, kl, residual)
+    compare(got, want, tol)
+
+
+@pytest.mark.parametrize('Sq', [1, 530])
+def test_offsets_beyond_32_bits(device, Sq):
+    """Rows just under 2^22 elements apart: 2^31 elements are passed by the 513th, 2^32 bytes too."""
+    H, Hkv, D, Sk, apart = 2, 1, 64, 530, 2 ** 22 - 8
+    q, k, v, do = make(device, 1, Sq, Sk, H, Hkv, D, 'bf16')
+    buf = torch.empty(Sk * apart, dtype=torch.bfloat16, device=device)
+    far, at = [], 0
+    for t in (q, k, v, do):
+        S, h = t.shape[1:3]
+        far.append(buf.as_strided((1, S, h, D), (8, apart, D, 1), at).copy_(t))
+        at += h * D
+    want = run(q, k, v, do, causal=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, run(*far, causal=True)))
+
+
+def test_two_calls_at_once(device):
+    """Calls in flight on two streams use workspaces of their own."""
+    sets = [make(device, 4, 96, 3000, 4, 2, 64, 'f32', seed=s) for s in (1, 2)]
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(run(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for a, b in zip(want, got) for x, y in zip(a, b))
