@@ -6,8 +6,9 @@
 //   dx = rstd (dz w_c - m1 - xhat m2),   m1, m2 = means over the group of dz w_c and dz w_c xhat
 //
 // Both directions are bound by memory.  A sample whose rows fit in the registers of one workgroup is read once and written
-// once (resident kernels); a larger one takes a pass for its sums, a small launch that finishes them, and a pass that
-// applies them.  Sums are kept per channel, so a group may end anywhere in a thread's vector of channels.
+// once (resident kernels; 800 x 196 x 64 fp32: 22 us forward, 30 backward, 3.6 and 4.0 TB/s); a larger one takes a pass for its
+// sums, a small launch that finishes them, and a pass that applies them (16 x 9216 x 320 bf16: 17 + 5 + 34 us forward, 41 + 6 +
+// 60 + 6 backward: 3.1 to 5.6 TB/s in the passes).  A thread's sums are per channel, so a group may end anywhere in its vector.
 //
 // The forward's sums of x and x^2 are fp64 (full rate on this card, and two instructions of the few per value): no
 // shift, no second pass, and a variance that survives a mean thousands of deviations away.  The mean is kept as two fp32
@@ -124,13 +125,19 @@ struct Channel {
     float mh[V], ml[V], rs[V], w[V], b[V];
 };
 template <int V>
-__device__ __forceinline__ void load_channels(const Args& a, const float4* st, int c0, Channel<V>& k) {
+__device__ __forceinline__ void load_params(const Args& a, int c0, Channel<V>& k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        k.w[j] = param(a.w, a.wtype, c0 + j, 1.f);
+        k.b[j] = param(a.b, a.wtype, c0 + j, 0.f);
+    }
+}
+template <int V>
+__device__ __forceinline__ void load_stats(const Args& a, const float4* st, int c0, Channel<V>& k) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float4 s = st[(c0 + j) / a.Cg];
         k.mh[j] = s.x; k.ml[j] = s.y; k.rs[j] = s.z;
-        k.w[j] = param(a.w, a.wtype, c0 + j, 1.f);
-        k.b[j] = param(a.b, a.wtype, c0 + j, 0.f);
     }
 }
 
@@ -152,14 +159,61 @@ __device__ __forceinline__ void forward_of(const Channel<V>& k, int act, float (
     activate<V>(x, act);
 }
 
+// ------------------------------------------------------------------------------------------------ sums where threads meet
+__device__ __forceinline__ double2 add2(double2 a, double2 b) { return make_double2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ double2 wide(double2 a) { return a; }
+__device__ __forceinline__ double2 wide(float2 a) { return make_double2((double)a.x, (double)a.y); }
+__device__ __forceinline__ void narrow(double2 a, double2& b) { b = a; }
+__device__ __forceinline__ void narrow(double2 a, float2& b) { b = make_float2((float)a.x, (float)a.y); }
+
+// column sums of red[rows][cols] into put(c, sum); called by all THREADS threads.  Where there are fewer columns than threads,
+// a column's rows are first shared out over `parts` threads, each of which leaves its sum in the first of its rows (one thread
+// per column took 29.9 us of the forward for 800 samples of 196 x 64 bf16 values: 64 rows one after the other).
+template <int THREADS, typename S, typename Put>
+__device__ __forceinline__ void column_sums(S* red, int rows, int cols, Put&& put) {
+    const int t = threadIdx.x;
+    int parts = min(THREADS / cols, rows);
+    if (parts > 1) {
+        const int j = t / cols, c = t - j * cols;
+        if (j < parts) {
+            double2 s = wide(red[j * cols + c]);
+            for (int r = j + parts; r < rows; r += parts) s = add2(s, wide(red[r * cols + c]));
+            narrow(s, red[j * cols + c]);
+        }
+        __syncthreads();
+    } else {
+        parts = rows;
+    }
+    for (int c = t; c < cols; c += THREADS) {
+        double2 s = wide(red[c]);
+        for (int r = 1; r < parts; ++r) s = add2(s, wide(red[r * cols + c]));
+        put(c, s);
+    }
+}
+
+// put(g, sum over i < items of get(g, i)) for each group, by as many lanes per group as there are
+template <int THREADS, typename Get, typename Put>
+__device__ __forceinline__ void group_sums(int G, int items, Get&& get, Put&& put) {
+    int L = 64;
+    while (L > 1 && L * G > THREADS) L >>= 1;
+    const int l = (int)threadIdx.x % L;
+    for (int g = (int)threadIdx.x / L; g < G; g += THREADS / L) {
+        double2 s = make_double2(0.0, 0.0);
+        for (int i = l; i < items; i += L) s = add2(s, get(g, i));
+        for (int o = L >> 1; o > 0; o >>= 1) s = add2(s, make_double2(__shfl_xor(s.x, o), __shfl_xor(s.y, o)));
+        if (l == 0) put(g, s);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ resident
 // One workgroup per sample; thread t holds vectors t, t + A, t + 2A ... of the sample's P * CV, A = the largest multiple
 // of CV up to the workgroup: its channels are the same in all of them.
 template <typename T, int V, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
-    double2* red = reinterpret_cast<double2*>(smem);                       // [rows][C], then [C]
-    float4* st = reinterpret_cast<float4*>(smem + (size_t)THREADS * V * sizeof(double2));
+    const bool one = a.Cg % V == 0;                                        // a thread's channels are of one group
+    double2* red = reinterpret_cast<double2*>(smem);                       // [rows][CV or C]
+    float4* st = reinterpret_cast<float4*>(smem + (size_t)THREADS * (one ? 1 : V) * sizeof(double2));
     typedef typename Vec<T, V>::type TV;
     const int n = blockIdx.x, t = threadIdx.x;
     const int rows = THREADS / a.CV, A = rows * a.CV;
@@ -188,34 +242,32 @@ __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
             }
         }
     }
-    if (on)
+    if (one) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) red[row * a.C + c0 + j] = make_double2(s1[j], s2[j]);
-    __syncthreads();
-    for (int c = t; c < a.C; c += THREADS) {
-        double2 s = red[c];
-        for (int r = 1; r < rows; ++r) {
-            const double2 q = red[r * a.C + c];
-            s.x += q.x;
-            s.y += q.y;
+        for (int j = 1; j < V; ++j) {
+            s1[0] += s1[j];
+            s2[0] += s2[j];
         }
-        red[c] = s;
+        if (on) red[t] = make_double2(s1[0], s2[0]);
+    } else if (on) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[t * V + j] = make_double2(s1[j], s2[j]);
     }
     __syncthreads();
-    for (int g = t; g < a.G; g += THREADS) {
-        double u = 0.0, v = 0.0;
-        for (int c = g * a.Cg; c < (g + 1) * a.Cg; ++c) {
-            u += red[c].x;
-            v += red[c].y;
-        }
-        const float4 s = make_stats(u, v, (double)a.P * a.Cg, a.eps);
-        st[g] = s;
-        if (a.stats) a.stats[(long)n * a.G + g] = s;
-    }
+    const int w = one ? a.Cg / V : a.Cg, pitch = one ? a.CV : a.C;
+    group_sums<THREADS>(a.G, rows * w, [&](int g, int i) {
+        const int r = i / w;
+        return red[r * pitch + g * w + i - r * w];
+    }, [&](int g, double2 u) {
+        const float4 q = make_stats(u.x, u.y, (double)a.P * a.Cg, a.eps);
+        st[g] = q;
+        if (a.stats) a.stats[(long)n * a.G + g] = q;
+    });
     __syncthreads();
     if (!on) return;
     Channel<V> k;
-    load_channels<V>(a, st, c0, k);
+    load_params<V>(a, c0, k);
+    load_stats<V>(a, st, c0, k);
     T* y = (T*)a.y + (long)n * a.P * a.C + c0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -252,9 +304,10 @@ __global__ __launch_bounds__(THREADS) void bwd_resident_kernel(Args a) {
         }
     }
     for (int g = t; g < a.G; g += THREADS) st[g] = a.stats[(long)n * a.G + g];
-    __syncthreads();
     Channel<V> k;
-    if (on) load_channels<V>(a, st, c0, k);
+    if (on) load_params<V>(a, c0, k);
+    __syncthreads();
+    if (on) load_stats<V>(a, st, c0, k);
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
@@ -276,28 +329,20 @@ __global__ __launch_bounds__(THREADS) void bwd_resident_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) red[row * a.C + c0 + j] = make_float2(s1[j], s2[j]);
     __syncthreads();
-    for (int c = t; c < a.C; c += THREADS) {
-        double u = 0.0, v = 0.0;
-        for (int r = 0; r < rows; ++r) {
-            const float2 q = red[r * a.C + c];
-            u += (double)q.x;
-            v += (double)q.y;
-        }
-        const float2 s = make_float2((float)u, (float)v);
-        red[c] = s;
-        if (a.bpart) a.bpart[(long)n * a.C + c] = s;
-    }
+    column_sums<THREADS>(red, rows, a.C, [&](int c, double2 u) {
+        const float2 q = make_float2((float)u.x, (float)u.y);
+        red[c] = q;
+        a.bpart[(long)n * a.C + c] = q;
+    });
     __syncthreads();
-    for (int g = t; g < a.G; g += THREADS) {
-        double u = 0.0, v = 0.0;
-        for (int c = g * a.Cg; c < (g + 1) * a.Cg; ++c) {
-            const double w = (double)param(a.w, a.wtype, c, 1.f);
-            u += w * (double)red[c].x;
-            v += w * (double)red[c].y;
-        }
+    group_sums<THREADS>(a.G, a.Cg, [&](int g, int i) {
+        const int c = g * a.Cg + i;
+        const double wt = (double)param(a.w, a.wtype, c, 1.f);
+        return make_double2(wt * (double)red[c].x, wt * (double)red[c].y);
+    }, [&](int g, double2 u) {
         const double m = (double)a.P * a.Cg;
-        mm[g] = make_float2((float)(u / m), (float)(v / m));
-    }
+        mm[g] = make_float2((float)(u.x / m), (float)(u.y / m));
+    });
     __syncthreads();
     if (!on) return;
     float m1[V], m2[V];
@@ -370,17 +415,8 @@ __global__ __launch_bounds__(256) void fwd_sums_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) red[threadIdx.x * V + j] = make_double2(s1[j], s2[j]);
     __syncthreads();
-    if (q.row != 0) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        double2 s = red[threadIdx.x * V + j];
-        for (int r = 1; r < q.rows; ++r) {
-            const double2 u = red[(threadIdx.x + r * q.cw) * V + j];
-            s.x += u.x;
-            s.y += u.y;
-        }
-        a.part[((long)q.n * a.pc + q.pc) * a.C + q.c0 + j] = s;
-    }
+    const int c0 = q.c0 - ((int)threadIdx.x - q.row * q.cw) * V;
+    column_sums<256>(red, q.rows, q.cw * V, [&](int c, double2 u) { a.part[((long)q.n * a.pc + q.pc) * a.C + c0 + c] = u; });
 }
 
 // sums u, v over the 256 threads of a workgroup, in thread 0
@@ -422,7 +458,8 @@ __global__ __launch_bounds__(256) void fwd_apply_kernel(Args a) {
     const Piece q = piece<V>(a);
     if (!q.on) return;
     Channel<V> k;
-    load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+    load_params<V>(a, q.c0, k);
+    load_stats<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
     const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
     T* y = (T*)a.y + (long)q.n * a.P * a.C + q.c0;
 #pragma unroll 4
@@ -444,7 +481,8 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
     if (q.on) {
         Channel<V> k;
-        load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+        load_params<V>(a, q.c0, k);
+        load_stats<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
         const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
         const T* dy = (const T*)a.dy + q.n * a.g_sn + q.c0;
 #pragma unroll 2
@@ -463,17 +501,10 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) red[threadIdx.x * V + j] = make_float2(s1[j], s2[j]);
     __syncthreads();
-    if (q.row != 0) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        double u = 0.0, v = 0.0;
-        for (int r = 0; r < q.rows; ++r) {
-            const float2 s = red[(threadIdx.x + r * q.cw) * V + j];
-            u += (double)s.x;
-            v += (double)s.y;
-        }
-        a.bpart[((long)q.n * a.pc + q.pc) * a.C + q.c0 + j] = make_float2((float)u, (float)v);
-    }
+    const int c0 = q.c0 - ((int)threadIdx.x - q.row * q.cw) * V;
+    column_sums<256>(red, q.rows, q.cw * V, [&](int c, double2 u) {
+        a.bpart[((long)q.n * a.pc + q.pc) * a.C + c0 + c] = make_float2((float)u.x, (float)u.y);
+    });
 }
 
 __global__ __launch_bounds__(256) void bwd_finish_kernel(Args a) {
@@ -499,7 +530,8 @@ __global__ __launch_bounds__(256) void bwd_apply_kernel(Args a) {
     const Piece q = piece<V>(a);
     if (!q.on) return;
     Channel<V> k;
-    load_channels<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
+    load_params<V>(a, q.c0, k);
+    load_stats<V>(a, a.stats + (long)q.n * a.G, q.c0, k);
     float m1[V], m2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -555,25 +587,30 @@ struct Plan {
     int pc, rows_per, cc;
 };
 
+// Channels per thread: four where addresses allow it (16-bit types: eight, in 16-byte loads, cost twice the registers per thread
+// and so half the workgroups: 66.9 us instead of 47.5 for 800 x 196 x 64 bf16 values forward and backward, 193 instead of 170
+// of kernels for 16 x 9216 x 320), two of a 16-bit type where only its pairs are aligned, else one.
 static int vec_of(const cmvae_group_norm& d, bool backward) {
-    const int full = d.dtype == CMVAE_F32 ? 4 : 8, es = d.dtype == CMVAE_F32 ? 4 : 2;
+    const int es = d.dtype == CMVAE_F32 ? 4 : 2;
     auto fits = [&](int v) {
         auto ok = [&](const void* p, const int64_t* s) { return (uintptr_t)p % (v * es) == 0 && s[0] % v == 0 && s[1] % v == 0; };
         const int64_t dense[2] = {0, 0};
         return d.C % v == 0 && ok(d.x, d.x_stride) &&
                (backward ? ok(d.dy, d.dy_stride) && ok(d.dx, dense) : ok(d.y, dense));
     };
-    if (fits(full)) return full;
-    if (full == 8 && fits(2)) return 2;
+    if (fits(4)) return 4;
+    if (es == 2 && fits(2)) return 2;
     return 1;
 }
 
-// Resident while a sample fits: 64 threads x 2 vectors, 256 x 2, 512 x 8, 1024 x 16 (forward; half in the backward,
-// which holds two tensors).
+// Resident while a sample fits: 64 threads x 4 vectors, 256 x 4, 512 x 8, 1024 x 16 (forward; half in the backward, which holds
+// two tensors).  Forward + backward in us, fp32, 64 channels, resident against in pieces: 4000 samples of 16 pixels 33 / 134, 800
+// of 196 55 / 89, 256 of 512 43 / 70; the forward of 256 of 1024 (1024 x 16) 29 / 42.  64 x 2 and 256 x 2: 47 for the 4000 of 16,
+// 35 instead of 27 for 800 of 64.
 static Plan plan_of(const cmvae_group_norm& d, int V, bool backward) {
     Plan p = {0, 0, 1, d.P, 1};
     const int CV = d.C / V;
-    const struct { int threads, r; } sizes[4] = {{64, 2}, {256, 2}, {512, 8}, {1024, backward ? 8 : 16}};
+    const struct { int threads, r; } sizes[4] = {{64, 4}, {256, 4}, {512, 8}, {1024, backward ? 8 : 16}};
     for (const auto& s : sizes) {
         if (CV > s.threads || d.G > 1024) continue;
         const int rows = s.threads / CV;
@@ -604,11 +641,11 @@ static size_t ws_bytes(const cmvae_group_norm& d, const Plan& p, bool backward) 
 template <typename T, int V>
 static int run_fwd(Args a, const Plan& p, void* stream) {
     if (p.threads) {
-        const size_t lds = (size_t)p.threads * V * sizeof(double2) + a.G * sizeof(float4);
+        const size_t lds = (size_t)p.threads * (a.Cg % V == 0 ? 1 : V) * sizeof(double2) + a.G * sizeof(float4);
         const char* what = "group_norm fwd_resident_kernel";
         switch (p.threads) {
-            case 64: return launch_kernel<fwd_resident_kernel<T, V, 64, 2>>(a.N, 64, lds, a, stream, what);
-            case 256: return launch_kernel<fwd_resident_kernel<T, V, 256, 2>>(a.N, 256, lds, a, stream, what);
+            case 64: return launch_kernel<fwd_resident_kernel<T, V, 64, 4>>(a.N, 64, lds, a, stream, what);
+            case 256: return launch_kernel<fwd_resident_kernel<T, V, 256, 4>>(a.N, 256, lds, a, stream, what);
             case 512: return launch_kernel<fwd_resident_kernel<T, V, 512, 8>>(a.N, 512, lds, a, stream, what);
             default: return launch_kernel<fwd_resident_kernel<T, V, 1024, 16>>(a.N, 1024, lds, a, stream, what);
         }
@@ -626,8 +663,8 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
         const size_t lds = (size_t)p.threads * V * sizeof(float2) + a.G * (sizeof(float4) + sizeof(float2));
         const char* what = "group_norm bwd_resident_kernel";
         switch (p.threads) {
-            case 64: e = launch_kernel<bwd_resident_kernel<T, V, 64, 2>>(a.N, 64, lds, a, stream, what); break;
-            case 256: e = launch_kernel<bwd_resident_kernel<T, V, 256, 2>>(a.N, 256, lds, a, stream, what); break;
+            case 64: e = launch_kernel<bwd_resident_kernel<T, V, 64, 4>>(a.N, 64, lds, a, stream, what); break;
+            case 256: e = launch_kernel<bwd_resident_kernel<T, V, 256, 4>>(a.N, 256, lds, a, stream, what); break;
             case 512: e = launch_kernel<bwd_resident_kernel<T, V, 512, 8>>(a.N, 512, lds, a, stream, what); break;
             default: e = launch_kernel<bwd_resident_kernel<T, V, 1024, 8>>(a.N, 1024, lds, a, stream, what);
         }
@@ -642,10 +679,10 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
     return check_launch("group_norm param_grad_kernel");
 }
 
-template <typename T, int FULL>
+template <typename T>
 static int run(const Args& a, const Plan& p, int V, bool backward, void* stream) {
-    if (V == FULL) return backward ? run_bwd<T, FULL>(a, p, stream) : run_fwd<T, FULL>(a, p, stream);
-    if constexpr (FULL == 8) {
+    if (V == 4) return backward ? run_bwd<T, 4>(a, p, stream) : run_fwd<T, 4>(a, p, stream);
+    if constexpr (sizeof(T) == 2) {
         if (V == 2) return backward ? run_bwd<T, 2>(a, p, stream) : run_fwd<T, 2>(a, p, stream);
     }
     return backward ? run_bwd<T, 1>(a, p, stream) : run_fwd<T, 1>(a, p, stream);
@@ -703,9 +740,9 @@ static int enter(const char* who, const cmvae_group_norm* d, bool backward, void
         if (!a.stats) a.stats = (float4*)(a.part + (size_t)d->N * p.pc * d->C);
     }
     switch (d->dtype) {
-        case CMVAE_F32: return run<float, 4>(a, p, V, backward, stream);
-        case CMVAE_BF16: return run<__bf16, 8>(a, p, V, backward, stream);
-        default: return run<_Float16, 8>(a, p, V, backward, stream);
+        case CMVAE_F32: return run<float>(a, p, V, backward, stream);
+        case CMVAE_BF16: return run<__bf16>(a, p, V, backward, stream);
+        default: return run<_Float16>(a, p, V, backward, stream);
     }
 }
 
