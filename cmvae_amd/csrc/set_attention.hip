@@ -22,6 +22,7 @@
 // 16-bit types P and dS are rounded once (to nearest) to be factors.
 #include "common.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -1285,33 +1286,87 @@ struct Plan {
     size_t lds;
 };
 
-// `rows` own rows in tiles of 32, `len` rows to walk; `occ` workgroups of four waves fit on a compute unit.  Four tiles of
-// own rows per workgroup share what they walk; where that leaves compute units without work, one tile per workgroup, whose
-// waves share out the walk.  The walk is cut into pieces, which a second launch joins, until there is a workgroup for every
-// slot — twice that for the causal order at one workgroup per unit (two are dealt in pairs, see place()), and half again as
-// much where lengths will leave some without work.
-static Plan make_plan(int esize, int D, long nbh, int rows, int len, bool stats, int occ, bool causal, bool ragged) {
+// One kernel's problem: `rows` own rows in tiles of 32 per (batch, key head), `len` rows to walk; `occ` workgroups of four
+// waves fit on a compute unit; `key_side`: dk and dv.
+struct Problem {
+    int esize, D;
+    long nbh;
+    int rows, len;
+    bool key_side;
+    int occ;
+    bool causal, ragged;
+    int walkers() const { return esize * D > 256 ? 2 : 4; }
+};
+
+static Plan plan_with(const Problem& x, int nw, int nsplit) {
     Plan p;
     p.piece = 0;
-    p.occ = occ;
-    const long wg4 = nbh * ((rows + 127) / 128), cus = compute_units();
-    p.nw = wg4 >= cus ? 4 : 1;
-    p.tile = p.nw == 4 && esize == 2 ? 64 : 32;
-    p.ntiles = (rows + 32 * p.nw - 1) / (32 * p.nw);
-    p.nsplit = 1;
-    const int tiles = (len + p.tile - 1) / p.tile, ws = esize * D > 256 ? 2 : 4;
-    const long wg = nbh * p.ntiles;
-    long want = p.nw == 4 ? cus * occ : cus;
-    if (p.nw == 4) want = causal && occ == 1 ? 2 * want : ragged ? want + want / 2 : want;
-    const int least = p.nw == 4 ? 4 : 2 * ws;      // tiles per piece
-    if (wg > 0 && wg < want && tiles >= 2 * least) {
-        long ns = (want + wg - 1) / wg;
-        if (ns > tiles / least) ns = tiles / least;
-        p.nsplit = (int)(ns > 64 ? 64 : ns);
-    }
-    const size_t buf = (size_t)2 * (esize == 4 ? 3 : 1) * p.tile * (D * 2 + 16) + (stats ? p.tile * 8 : 0);
-    p.lds = (p.nw == 4 ? 2 : ws) * buf;
+    p.occ = x.occ;
+    p.nw = nw;
+    p.nsplit = nsplit;
+    p.tile = nw == 4 && x.esize == 2 ? 64 : 32;
+    p.ntiles = (x.rows + 32 * nw - 1) / (32 * nw);
+    const size_t buf = (size_t)2 * (x.esize == 4 ? 3 : 1) * p.tile * (x.D * 2 + 16) + (x.key_side ? p.tile * 8 : 0);
+    p.lds = (nw == 4 ? 2 : x.walkers()) * buf;
     return p;
+}
+
+// What a plan takes, in us, by single launches: a four-wave workgroup alone on its compute unit takes 1.4 us per tile (16-bit
+// types, heads of 64) or 2 (fp32), twice that for heads of 128, and one tile's time for its ends; more workgroups on a unit add
+// `more` of that each.  A round of waves that share out a walk takes `round` tiles, their ends and their meeting `ends`.  A
+// joining launch: 4 us and the pieces' results, written and read at 4 TB/s.
+static double cost(const Problem& x, const Plan& p) {
+    const bool half = x.esize == 2;
+    const double tau = (half ? 1.4 : 2.0) * (x.D / 64);
+    const double more = p.nw == 1 ? (half && x.D == 64 ? 0.6 : 1.0) : p.occ == 1 ? 1.0 : half ? 0.55 : 0.78;
+    const double round = half ? 0.65 : 1.0, ends = half ? 2.2 : 3.5;
+    const int per = ((x.len + p.tile - 1) / p.tile + p.nsplit - 1) / p.nsplit;
+    const double load = (double)(x.nbh * p.ntiles * p.nsplit) / compute_units();
+    const double turns = more * (x.causal || x.ragged ? 0.6 * load + 0.4 : std::ceil(load));     // uneven ones fill each other's gaps
+    const double one = p.nw == 4 ? per + 1 : (per + x.walkers() - 1) / x.walkers() * round + ends;
+    const double bytes = 8.0 * p.nsplit * x.nbh * x.rows * x.D * (x.key_side ? 2 : 1);
+    return tau * one * (turns > 1.0 ? turns : 1.0) + (p.nsplit > 1 ? 4.0 + bytes / 4e6 : 0.0);
+}
+
+// Four tiles of own rows per workgroup share what they walk; or one tile per workgroup, whose waves share out the walk.  The
+// walk may be cut into pieces, which a second launch joins.
+//   Where four tiles per workgroup fill the card: those, with pieces until there is a workgroup for every slot — twice that for
+//   the causal order at one workgroup per unit (two are dealt in pairs, see place()), and half again as much where lengths will
+//   leave some without work.
+//   Else whatever costs least of both kinds, whole or in as many pieces as one, two or three turns of the card hold.  Forward +
+//   backward in us, four tiles against one: fp32 4 x 200 rows x 4 heads of 64 67 / 43, 16 x 300 106 / 146, 400 against 8000
+//   141 / 270, causal 4096 x 2 heads of 128 416 / 1261; bf16 32 / 24, 39 / 55, 65 / 78, 160 / 206.
+static Plan make_plan(const Problem& x) {
+    const long cus = compute_units();
+    Plan best = plan_with(x, 4, 1);
+    const long wg4 = x.nbh * best.ntiles;
+    if (wg4 >= cus) {
+        const int tiles = (x.len + best.tile - 1) / best.tile;
+        const long slots = cus * x.occ, want = x.causal && x.occ == 1 ? 2 * slots : x.ragged ? slots + slots / 2 : slots;
+        if (wg4 < want && tiles >= 8) {
+            const long ns = (want + wg4 - 1) / wg4;
+            best.nsplit = (int)(ns > tiles / 4 ? tiles / 4 : ns);
+        }
+        return best;
+    }
+    if (wg4 == 0) return best;
+    double least = cost(x, best);
+    for (const int nw : {4, 1}) {
+        Plan p = plan_with(x, nw, 1);
+        const long wg = x.nbh * p.ntiles, tiles = (x.len + p.tile - 1) / p.tile;
+        const long most = std::min(64L, nw == 4 ? tiles / 2 : tiles / (2 * x.walkers()));
+        for (int turn = 0; turn <= 3; ++turn) {
+            const long ns = turn == 0 ? 1 : std::min(most, turn * cus / wg);
+            if (turn > 0 && ns <= p.nsplit) continue;
+            p.nsplit = (int)ns;
+            const double c = cost(x, p);
+            if (c < least) {
+                least = c;
+                best = p;
+            }
+        }
+    }
+    return best;
 }
 
 // Few rows: four waves per workgroup, at least two rounds of 16-byte loads each per piece, eight workgroups per unit (of padded lists some have no keys: 4 82 us, 8 76, 16 79 at 16 lists of up to 8191 keys x 8 heads of 128).
@@ -1341,9 +1396,10 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const long nbh = (long)d.B * d.Hkv;
     const int R = G * d.Sq;
     const bool causal = d.causal != 0, ragged = d.q_len || d.k_len;
-    z.f = R <= 8 ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
-    z.q = make_plan(es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged);
-    z.k = make_plan(es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged);
+    const Problem qside = {es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged};
+    z.f = R <= 8 ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(qside);
+    z.q = make_plan(qside);
+    z.k = make_plan({es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged});
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
     z.fwd = z.f.nsplit > 1 ? z.f.nsplit * rows * (d.D + 2) * 4 : 0;
     const size_t bq = z.q.nsplit > 1 ? z.q.nsplit * rows * d.D * 4 : 0;
