@@ -7,8 +7,8 @@
 //
 // Both directions are bound by memory.  A sample whose rows fit in the registers of one workgroup is read once and written
 // once (resident kernels; 800 x 196 x 64 fp32: 22 us forward, 30 backward, 3.6 and 4.0 TB/s); a larger one takes a pass for its
-// sums, a small launch that finishes them, and a pass that applies them (16 x 9216 x 320 bf16: 17 + 5 + 34 us forward, 41 + 6 +
-// 60 + 6 backward: 3.1 to 5.6 TB/s in the passes).  A thread's sums are per channel, so a group may end anywhere in its vector.
+// sums, a small launch that finishes them, and a pass that applies them (16 x 9216 x 320 bf16: 64 us forward, 108 backward, 4.4
+// TB/s over what the passes move).  A thread's sums are per channel, so a group may end anywhere in its vector.
 //
 // The forward's sums of x and x^2 are fp64 (full rate on this card, and two instructions of the few per value): no
 // shift, no second pass, and a variance that survives a mean thousands of deviations away.  The mean is kept as two fp32
@@ -31,7 +31,7 @@ struct Args {
     float2* means;                              // m1, m2 [N, G]
     long x_sn, x_sp, g_sn, g_sp;                // strides in elements
     int N, P, C, G, Cg, CV, act, wtype;
-    int pc, rows_per, cc;                       // pixel pieces per sample, pixels per piece, channel pieces
+    int pc, rows_per, cc, cw;                   // pixel pieces per sample, pixels per piece, channel pieces, vectors per one
     float eps;
 };
 
@@ -381,11 +381,11 @@ __device__ __forceinline__ Piece piece(const Args& a) {
     id /= a.cc;
     q.pc = id % a.pc;
     q.n = id / a.pc;
-    q.cw = min(a.CV - cc * 256, 256);                             // vectors of channels in this piece
+    q.cw = min(a.CV - cc * a.cw, a.cw);                           // vectors of channels in this piece
     q.rows = 256 / q.cw;
     q.row = (int)threadIdx.x / q.cw;
     q.on = q.row < q.rows;
-    q.c0 = (cc * 256 + (int)threadIdx.x - q.row * q.cw) * V;
+    q.c0 = (cc * a.cw + (int)threadIdx.x - q.row * q.cw) * V;
     q.p0 = q.pc * a.rows_per;
     q.p1 = min(a.P, q.p0 + a.rows_per);
     return q;
@@ -419,37 +419,37 @@ __global__ __launch_bounds__(256) void fwd_sums_kernel(Args a) {
     column_sums<256>(red, q.rows, q.cw * V, [&](int c, double2 u) { a.part[((long)q.n * a.pc + q.pc) * a.C + c0 + c] = u; });
 }
 
-// sums u, v over the 256 threads of a workgroup, in thread 0
-__device__ __forceinline__ void block_sum(double& u, double& v) {
-    __shared__ double2 red[4];
+// Sum over `rows` rows, `pitch` apart, of `width` neighbours of part (each times weight(i), i < width), in thread 0 of a
+// workgroup of FIN threads: lanes beside each other take neighbours, four loads in flight each.
+template <int FIN, typename S, typename W>
+__device__ __forceinline__ double2 block_sum(const S* part, int rows, long pitch, int width, W&& weight) {
+    __shared__ double2 red[FIN / 64];
+    double2 s = make_double2(0.0, 0.0);
+    const int across = min(width, FIN), step = FIN / across, r0 = (int)threadIdx.x / across;
+    if (r0 < step)
+        for (int c = (int)threadIdx.x - r0 * across; c < width; c += across) {
+            double2 u = make_double2(0.0, 0.0);
+#pragma unroll 4
+            for (int r = r0; r < rows; r += step) u = add2(u, wide(part[r * pitch + c]));
+            const double w = weight(c);
+            s = add2(s, make_double2(w * u.x, w * u.y));
+        }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        u += __shfl_xor(u, o);
-        v += __shfl_xor(v, o);
-    }
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_double2(u, v);
+    for (int o = 32; o > 0; o >>= 1) s = add2(s, make_double2(__shfl_xor(s.x, o), __shfl_xor(s.y, o)));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0)
-        for (int i = 1; i < 4; ++i) {
-            u += red[i].x;
-            v += red[i].y;
-        }
+        for (int i = 1; i < FIN / 64; ++i) s = add2(s, red[i]);
+    return s;
 }
 
 // one workgroup per (sample, group)
-__global__ __launch_bounds__(256) void fwd_finish_kernel(Args a) {
+template <int FIN>
+__global__ __launch_bounds__(FIN) void fwd_finish_kernel(Args a) {
     const long ng = blockIdx.x;
     const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
-    double u = 0.0, v = 0.0;
-    const int items = a.pc * a.Cg;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const int pc = i / a.Cg, c = i - pc * a.Cg;
-        const double2 s = a.part[((long)n * a.pc + pc) * a.C + g * a.Cg + c];
-        u += s.x;
-        v += s.y;
-    }
-    block_sum(u, v);
-    if (threadIdx.x == 0) a.stats[ng] = make_stats(u, v, (double)a.P * a.Cg, a.eps);
+    const double2 s = block_sum<FIN>(a.part + (long)n * a.pc * a.C + g * a.Cg, a.pc, a.C, a.Cg, [](int) { return 1.0; });
+    if (threadIdx.x == 0) a.stats[ng] = make_stats(s.x, s.y, (double)a.P * a.Cg, a.eps);
 }
 
 template <typename T, int V>
@@ -507,21 +507,14 @@ __global__ __launch_bounds__(256) void bwd_sums_kernel(Args a) {
     });
 }
 
-__global__ __launch_bounds__(256) void bwd_finish_kernel(Args a) {
+template <int FIN>
+__global__ __launch_bounds__(FIN) void bwd_finish_kernel(Args a) {
     const long ng = blockIdx.x;
     const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
-    double u = 0.0, v = 0.0;
-    const int items = a.pc * a.Cg;
-    for (int i = threadIdx.x; i < items; i += 256) {
-        const int pc = i / a.Cg, c = g * a.Cg + i - pc * a.Cg;
-        const float2 s = a.bpart[((long)n * a.pc + pc) * a.C + c];
-        const double w = (double)param(a.w, a.wtype, c, 1.f);
-        u += w * (double)s.x;
-        v += w * (double)s.y;
-    }
-    block_sum(u, v);
+    const double2 s = block_sum<FIN>(a.bpart + (long)n * a.pc * a.C + g * a.Cg, a.pc, a.C, a.Cg,
+                                [&](int c) { return (double)param(a.w, a.wtype, g * a.Cg + c, 1.f); });
     const double m = (double)a.P * a.Cg;
-    if (threadIdx.x == 0) a.means[ng] = make_float2((float)(u / m), (float)(v / m));
+    if (threadIdx.x == 0) a.means[ng] = make_float2((float)(s.x / m), (float)(s.y / m));
 }
 
 template <typename T, int V>
@@ -584,12 +577,12 @@ __global__ __launch_bounds__(256) void param_grad_kernel(Args a, long items) {
 // ------------------------------------------------------------------------------------------------ launches
 struct Plan {
     int threads, r;                             // resident: threads per sample and vectors per thread; 0: in pieces
-    int pc, rows_per, cc;
+    int pc, rows_per, cc, cw;
 };
 
 // Channels per thread: four where addresses allow it (16-bit types: eight, in 16-byte loads, cost twice the registers per thread
 // and so half the workgroups: 66.9 us instead of 47.5 for 800 x 196 x 64 bf16 values forward and backward, 193 instead of 170
-// of kernels for 16 x 9216 x 320), two of a 16-bit type where only its pairs are aligned, else one.
+// of kernels for 16 x 9216 x 320), two where only pairs are aligned, else one.
 static int vec_of(const cmvae_group_norm& d, bool backward) {
     const int es = d.dtype == CMVAE_F32 ? 4 : 2;
     auto fits = [&](int v) {
@@ -599,7 +592,7 @@ static int vec_of(const cmvae_group_norm& d, bool backward) {
                (backward ? ok(d.dy, d.dy_stride) && ok(d.dx, dense) : ok(d.y, dense));
     };
     if (fits(4)) return 4;
-    if (es == 2 && fits(2)) return 2;
+    if (fits(2)) return 2;
     return 1;
 }
 
@@ -608,7 +601,7 @@ static int vec_of(const cmvae_group_norm& d, bool backward) {
 // of 196 55 / 89, 256 of 512 43 / 70; the forward of 256 of 1024 (1024 x 16) 29 / 42.  64 x 2 and 256 x 2: 47 for the 4000 of 16,
 // 35 instead of 27 for 800 of 64.
 static Plan plan_of(const cmvae_group_norm& d, int V, bool backward) {
-    Plan p = {0, 0, 1, d.P, 1};
+    Plan p = {0, 0, 1, d.P, 1, 0};
     const int CV = d.C / V;
     const struct { int threads, r; } sizes[4] = {{64, 4}, {256, 4}, {512, 8}, {1024, backward ? 8 : 16}};
     for (const auto& s : sizes) {
@@ -620,9 +613,13 @@ static Plan plan_of(const cmvae_group_norm& d, int V, bool backward) {
             return p;
         }
     }
-    p.cc = (CV + 255) / 256;
-    const int cw = CV < 256 ? CV : 256, rows = 256 / cw;
-    const long target = 2048, have = (long)d.N * p.cc;
+    // In pieces: six workgroups per unit (3 x 16000 x 1280 bf16, forward + backward: 200 us; four 221, eight 229), of 64 vectors of
+    // channels or 128 narrow ones, evenly shared out, and the rest in rows (256 and 6: 226).
+    const int widest = V == 4 ? 64 : 128;
+    p.cc = (CV + widest - 1) / widest;
+    p.cw = (CV + p.cc - 1) / p.cc;
+    const int rows = 256 / p.cw;
+    const long target = 6L * compute_units(), have = (long)d.N * p.cc;
     long pc = (target + have - 1) / have;
     const long most = (d.P + 4L * rows - 1) / (4L * rows);          // at least four pixels per thread
     if (pc > most) pc = most;
@@ -636,6 +633,15 @@ static size_t ws_bytes(const cmvae_group_norm& d, const Plan& p, bool backward) 
     const size_t nc = (size_t)d.N * p.pc * d.C;
     if (!backward) return p.threads ? 0 : nc * sizeof(double2) + (size_t)d.N * d.G * sizeof(float4);
     return nc * sizeof(float2) + 256 + (size_t)d.N * d.G * sizeof(float2);
+}
+
+// One wave per (sample, group) while a lane has at most 16 values to add, else sixteen (the backward of 1000 samples of 30 x 1280
+// bf16 values, 32 groups: 95 us by one, 241 by sixteen; forward + backward of one of 16384 x 1280: 88 by sixteen, 229 by four).
+template <void (*WAVE)(Args), void (*WIDE)(Args)>
+static int finish(const Args& a, void* stream, const char* what) {
+    const long blocks = (long)a.N * a.G;
+    return (long)a.pc * a.Cg <= 1024 ? launch_kernel<WAVE>(blocks, 64, 0, a, stream, what)
+                                     : launch_kernel<WIDE>(blocks, 1024, 0, a, stream, what);
 }
 
 template <typename T, int V>
@@ -652,7 +658,7 @@ static int run_fwd(Args a, const Plan& p, void* stream) {
     }
     const long blocks = (long)a.N * a.pc * a.cc;
     if (int e = launch_kernel<fwd_sums_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm fwd_sums_kernel")) return e;
-    if (int e = launch_kernel<fwd_finish_kernel>((long)a.N * a.G, 256, 0, a, stream, "group_norm fwd_finish_kernel")) return e;
+    if (int e = finish<fwd_finish_kernel<64>, fwd_finish_kernel<1024>>(a, stream, "group_norm fwd_finish_kernel")) return e;
     return launch_kernel<fwd_apply_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm fwd_apply_kernel");
 }
 
@@ -671,7 +677,7 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
     } else {
         const long blocks = (long)a.N * a.pc * a.cc;
         if ((e = launch_kernel<bwd_sums_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm bwd_sums_kernel"))) return e;
-        if ((e = launch_kernel<bwd_finish_kernel>((long)a.N * a.G, 256, 0, a, stream, "group_norm bwd_finish_kernel"))) return e;
+        if ((e = finish<bwd_finish_kernel<64>, bwd_finish_kernel<1024>>(a, stream, "group_norm bwd_finish_kernel"))) return e;
         e = launch_kernel<bwd_apply_kernel<T, V>>(blocks, 256, 0, a, stream, "group_norm bwd_apply_kernel");
     }
     if (e || (!a.dw && !a.db)) return e;
@@ -682,9 +688,7 @@ static int run_bwd(Args a, const Plan& p, void* stream) {
 template <typename T>
 static int run(const Args& a, const Plan& p, int V, bool backward, void* stream) {
     if (V == 4) return backward ? run_bwd<T, 4>(a, p, stream) : run_fwd<T, 4>(a, p, stream);
-    if constexpr (sizeof(T) == 2) {
-        if (V == 2) return backward ? run_bwd<T, 2>(a, p, stream) : run_fwd<T, 2>(a, p, stream);
-    }
+    if (V == 2) return backward ? run_bwd<T, 2>(a, p, stream) : run_fwd<T, 2>(a, p, stream);
     return backward ? run_bwd<T, 1>(a, p, stream) : run_fwd<T, 1>(a, p, stream);
 }
 
@@ -715,7 +719,7 @@ static Args args_of(const cmvae_group_norm& d, const Plan& p, int V) {
     a.g_sn = d.dy_stride[0]; a.g_sp = d.dy_stride[1];
     a.N = d.N; a.P = d.P; a.C = d.C; a.G = d.G; a.Cg = d.C / d.G; a.CV = d.C / V;
     a.act = d.act; a.wtype = d.wdtype; a.eps = d.eps;
-    a.pc = p.pc; a.rows_per = p.rows_per; a.cc = p.cc;
+    a.pc = p.pc; a.rows_per = p.rows_per; a.cc = p.cc; a.cw = p.cw;
     return a;
 }
 
