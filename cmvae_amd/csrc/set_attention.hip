@@ -657,7 +657,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
 }
 
 // ------------------------------------------------------------------------------------------------ forward of few rows
-// A key head's list of at most 8 rows (one new token of grouped heads, a set's summary by one query) against many keys: the
+// A key head's list of a few rows (one new token, a set's summary by one query; most_rows()) against many keys: the
 // keys and values are read once, and that is the time.  No LDS, no matrix instruction (32 columns of which 1 .. 8 count):
 // a row of keys lies over CL lanes, 16 bytes each, 64 / CL keys per wave and step, U steps' loads in flight; a score is the
 // sum over the CL lanes, a lane keeps its channels' sums for its keys and its own running maximum, and the waves join at the
@@ -1369,7 +1369,14 @@ static Plan make_plan(const Problem& x) {
     return best;
 }
 
-// Few rows: four waves per workgroup, at least two rounds of 16-byte loads each per piece, eight workgroups per unit (of padded lists some have no keys: 4 82 us, 8 76, 16 79 at 16 lists of up to 8191 keys x 8 heads of 128).
+// Rows per key head up to which fwd_rows_kernel takes a list: its arithmetic grows with the rows, the matrix instructions' does
+// not.  Rows kernel / the other, us, for 16 lists of 8191 keys x 8 heads: bf16 heads of 128, 1 row 102 / 103, 2 103 / 102, 4 112 /
+// 105, 8 156 / 103; fp32 heads of 64, 4 rows 108 / 107 and for 16 of 2000 30 / 34 (6 rows 58 / 35); fp32 heads of 128, 1 row 193 /
+// 332, 8 262 / 330; one list of 8192 keys x 8 heads of 128, 1 row, bf16 10 / 14.
+constexpr int most_rows(int esize, int D) { return esize == 2 ? 2 : D == 64 ? 4 : 8; }
+
+// Few rows: four waves per workgroup, at least two rounds of 16-byte loads each per piece, eight workgroups per unit (of padded
+// lists some have no keys: 16 of up to 8191 keys x 8 heads of 128, 4 rows, 4 per unit 82 us, 8 76, 16 79).
 static Plan rows_plan(int esize, int D, long nbh, int len) {
     Plan p = {4, 0, 1, 1, 4, 0, 0};
     const int round = 4 * 4 * (64 / (D * esize / 16));           // keys per round of a workgroup
@@ -1397,7 +1404,7 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const int R = G * d.Sq;
     const bool causal = d.causal != 0, ragged = d.q_len || d.k_len;
     const Problem qside = {es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged};
-    z.f = R <= 8 ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(qside);
+    z.f = R <= most_rows(es, d.D) ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(qside);
     z.q = make_plan(qside);
     z.k = make_plan({es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged});
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
@@ -1430,13 +1437,18 @@ static int run_fwd(Args a, const Sizes& z, float* ws, void* stream) {
     a.part = ws;
     a.part_ml = ws + (size_t)a.nsplit * rows * D;
     const long blocks = nbh * a.ntiles * a.nsplit;
-    const char* what = "set_attention fwd_rows_kernel";
-    int e = a.R == 1 ? launch_kernel<fwd_rows_kernel<T, D, 1>>(blocks, 256, 0, a, stream, what)
-            : a.R == 2 ? launch_kernel<fwd_rows_kernel<T, D, 2>>(blocks, 256, 0, a, stream, what)
-            : a.R <= 4 ? launch_kernel<fwd_rows_kernel<T, D, 4>>(blocks, 256, 0, a, stream, what)
-            : a.R <= 8 ? launch_kernel<fwd_rows_kernel<T, D, 8>>(blocks, 256, 0, a, stream, what)
-            : z.f.nw == 4 ? launch_kernel<fwd_kernel<T, D, 4, T4, 1>>(blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
+    constexpr int MOST = most_rows(sizeof(T), D);
+    auto rows_of = [&](auto r) { return launch_kernel<fwd_rows_kernel<T, D, r>>(blocks, 256, 0, a, stream, "set_attention fwd_rows_kernel"); };
+    int e;
+    if (a.R <= MOST) {
+        if (a.R == 1) e = rows_of(std::integral_constant<int, 1>());
+        else if (a.R == 2) e = rows_of(std::integral_constant<int, 2>());
+        else if (a.R <= 4) e = rows_of(std::integral_constant<int, std::min(4, MOST)>());
+        else e = rows_of(std::integral_constant<int, MOST>());
+    } else {
+        e = z.f.nw == 4 ? launch_kernel<fwd_kernel<T, D, 4, T4, 1>>(blocks, 256, z.f.lds, a, stream, "set_attention fwd_kernel")
                         : launch_kernel<fwd_kernel<T, D, 1, 32, WS>>(blocks, WS * 64, z.f.lds, a, stream, "set_attention fwd_kernel");
+    }
     if (e || a.nsplit == 1) return e;
     a.sg = join_groups(a.nsplit, rows * (D / 4), 256 / (D / 4));
     return launch_kernel<fwd_join_kernel<T, D>>((rows * (D / 4) * a.sg + 255) / 256, 256, 0, a, stream, "set_attention fwd_join_kernel");
