@@ -19,7 +19,7 @@
 // bf16 pieces (to nearest, 8 + 8 + 8 bits) and each product as the six piece products that reach above 2^-24 of it —
 // fp32's own accuracy (test_gpu_set_attention.py holds it to fp32 tolerances) at 6/16 of the fp32 instruction's cycles.  An
 // infinite fp32 input makes NaN of its rows.  Scores, softmax statistics, delta and every accumulator are fp32; in the
-// 16-bit types P and dS are rounded once (to nearest) to be factors.
+// 16-bit types P and dS are rounded once (to nearest) to be factors, dq's dS into two.
 #include "common.h"
 
 #include <algorithm>
@@ -165,7 +165,11 @@ __device__ __forceinline__ f32x16 mul_rows(const char* tile, int row0, const Fra
 // Register r of the accumulator is tile row acc_row(r, h), which fixes the contraction's order: registers 8s .. 8s + 7 are
 // one instruction's eight; the matching first factor — four rows at one channel, twice — comes from the transposing LDS
 // read (16 lanes name 4 rows x 16 channels, lane i receives channel i of the four rows).
-template <typename T, int D, int ROWS>
+//   LOW (16-bit types): what the accumulator's rounding leaves is a factor of its own.  dq takes it: a row's sum over dS k
+// cancels what the keys have in common, the roundings of dS do not, and dq's error was 1.52 times that of its own rounding —
+// 1.06 with it, for a third more matrix instructions (dq of dense 8 x 4096 x 16 heads of 64 bf16 1018 -> 1142 us).  dk and dv, summed
+// over many queries, are at 1.4 without.
+template <typename T, int D, int ROWS, bool LOW = false>
 __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, const Sel& sel, f32x16 (&acc)[D / 32]) {
     constexpr int P = Elem<T>::P;
     typedef __attribute__((address_space(3))) s16x4 lds4;
@@ -173,7 +177,7 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
     const char* p = tile + (row0 + 4 * h + (i >> 2)) * pitch<D>() + (lane & 16) * 2 + (i & 3) * 8;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        u32x4 b[P];
+        u32x4 b[P], low[P];
         if constexpr (P == 3) {
             float v[8];
 #pragma unroll
@@ -184,6 +188,11 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = (T)w[8 * s + j];
             b[0] = __builtin_bit_cast(u32x4, v);
+            if constexpr (LOW) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (T)(w[8 * s + j] - (float)v[j]);
+                low[0] = __builtin_bit_cast(u32x4, v);
+            }
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
@@ -196,6 +205,7 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
                 a[k] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
             acc[d] = mma<T>(a, b, acc[d]);
+            if constexpr (LOW && P == 1) acc[d] = mma<T>(a, low, acc[d]);
         }
     }
 }
@@ -280,7 +290,7 @@ __device__ __forceinline__ f32x4 load4(const char* p) {
 }
 
 // one piece of a result row: o without the residual (16-bit types: and what its rounding leaves, so that the backward's delta is
-// not that of a rounded o — dq's error is then 1.4 times its own rounding's, not 1.53), and o
+// not that of a rounded o — dk's error is then 1.43 times its own rounding's, not 1.47, and dq's 1.06, not 1.19), and o
 template <typename T>
 __device__ __forceinline__ void store_o(const Args& a, long at, const char* residual, f32x4 o) {
     if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
@@ -998,7 +1008,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
                 for (int i = 0; i < 16; ++i)
                     if (k0 + u * 32 + acc_row(i, h) >= klast) s[i] = 0.f;
             }
-            mul_cols<T, D, KT>(kt, u * 32, s, sel, acc);
+            mul_cols<T, D, KT, true>(kt, u * 32, s, sel, acc);
         }
     };
     if constexpr (WS > 1) {
