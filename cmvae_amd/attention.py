@@ -22,7 +22,11 @@ def set_attention(q, k, v, scale=None, causal=False, q_len=None, k_len=None, res
     (padded batches; values are clamped to [0, S]); output rows behind q_len and all gradients of rows behind a length
     are zeros, and what such rows hold is never read.  causal: query i sees keys j <= i + k_len - q_len.  A query that
     sees no key gets zeros (plus its own row if `residual`).  Differentiable once in q, k, v; every result is the same
-    bits on every run."""
+    bits on every run.
+
+    Probabilities are fp32 and carry a relative error of 2^-24 of their row's largest score; 16-bit types round them once more
+    as factors.  A key that is NaN or infinite may reach any row of its batch entry, also those that the causal order hides
+    it from; an infinite float32 value makes NaN.  Scores beyond 2^22 are out of range in float16."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None and q.shape[-1] else scale
     if ops.CHECK_INDICES:
         for t, n, x in ((q_len, 'q_len', q), (k_len, 'k_len', k)):

@@ -303,7 +303,7 @@ __device__ __forceinline__ void store_o(const Args& a, long at, const char* resi
 // ---- tiles of ROWS rows through registers into LDS: requested while the previous tile is used -----------------------
 // A thread's pieces lie STEP rows apart, so their addresses are one 32-bit offset per thread on top of a scalar base (with a
 // 64-bit product per piece and tile instead, and a division per piece on the key side, dk and dv of dense 8 x 4096 x 16 heads
-// of 64 took @A@ us for @B@).
+// of 64 bf16 took 1579 us for 1380).
 template <typename T, int D, int ROWS, int THREADS>
 struct Stage {
     static constexpr int CPR = D * sizeof(T) / 16;               // 16-byte pieces per row
@@ -376,8 +376,8 @@ struct Place {           // what a workgroup works on
 //   Otherwise: (batch, key head) runs fastest — with a multiple of 8 of them each stays on one XCD, whose L2 then holds its
 //   keys — and the causal order's longest tiles come first.
 // With one to two workgroups per compute unit the second ones are dealt shortest first: each joins a long one.
-// Measured on 16 padded sets of 383 to 1531 rows, fp32, against plain order: forward 371 -> @F@ us, dq 522 -> @Q@, dk and dv
-// 690 -> @K@.
+// Measured on 16 padded sets of 383 to 1531 rows, fp32, against plain order: forward 371 -> 229 us, dq 522 -> 312, dk and dv
+// 690 -> 484.
 template <int ROWS, bool KEYS>
 __device__ __forceinline__ Place place(const Args& a) {
     Place p;
@@ -498,8 +498,12 @@ __device__ __forceinline__ void take_over(const char* smem, int w, float f, f32x
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Keys in tiles of KT through LDS.  Running maximum m (log2 units) and sum l per row.
-// nsplit > 1: a workgroup covers split_tiles tiles and leaves (acc, m, l) for the joining kernel.
+// Keys in tiles of KT through LDS.  Running maximum m (log2 units) and sum l per row.  nsplit > 1: a workgroup covers one
+// piece of the tiles and leaves (acc, m, l) for the joining kernel.
+//   Bound by the matrix instructions and, between them, the exponentials and the LDS reads that feed them: with two workgroups
+// per unit one computes while the other waits.  Dense 8 x 4096 x 16 heads, bf16: 700 TFLOP/s with 64 channels, 750 with 128 (a
+// large library product reaches 1130); fp32 (six bf16 products each), 8 x 2048 x 8 heads: 173 and 150 (the library's fp32
+// product 153).
 template <typename T, int D, int NW, int KT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -672,7 +676,8 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
 // a row of keys lies over CL lanes, 16 bytes each, 64 / CL keys per wave and step, U steps' loads in flight; a score is the
 // sum over the CL lanes, a lane keeps its channels' sums for its keys and its own running maximum, and the waves join at the
 // end.  16-bit values meet in v_dot2 (two products per instruction): scores over channel pairs, sums over pairs of keys.
-// A workgroup takes `piece` keys; pieces of a list are joined by fwd_join_kernel.
+// A workgroup takes `piece` keys; pieces of a list are joined by fwd_join_kernel.  Reads 5.3 TB/s at 16 lists of 8191 keys x 8 heads
+// of 128 (bf16 and fp32), 4.7 at 4 of 6400 x 4 heads of 64 fp32 (11 us).
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
@@ -939,7 +944,9 @@ __device__ __forceinline__ bool join_sum(const Args& a, const float* part, long 
 }
 
 // ------------------------------------------------------------------------------------------------ backward, query side
-// The forward's shape; delta_i from the saved o, kept for the key side.
+// The forward's shape; delta_i from the saved o, kept for the key side.  Bound as the forward; at its dense sizes, counting three
+// products, bf16 720 TFLOP/s with 64 channels and 740 with 128 (its fourth product, of what dS's rounding leaves, not counted),
+// fp32 203 and 175.
 template <typename T, int D, int NW, int KT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -1084,7 +1091,11 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward, key side
-// 32 keys per wave; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.
+// 32 keys per wave; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.  Bound as the
+// others, and with 128 channels by its registers: 128 accumulators and 128 of fragments leave one wave per SIMD, which waits out
+// its LDS reads itself (bf16, dense 8 x 4096 x 16 heads: 800 TFLOP/s with 64 channels, 600 with 128; fp32, 8 x 2048 x 8: 205 and
+// 170).  Not faster there: fragments requested a step ahead (600 -> 618, but 64 channels lose as much), tiles without padding in
+// a swizzled order (a third fewer bank conflicts, same time), dk and dv in workgroups of their own (548).
 template <typename T, int D, int NW, int RT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (sizeof(T) == 4 && D == 64)) ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];

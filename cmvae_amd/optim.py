@@ -2,7 +2,7 @@
 
 `linear.FlatAdam` is the reference's optimizer (L2 added to the gradient, one flat fp32 buffer; omniglot/trainer.py:48-52);
 `AdamW` decouples the weight decay, takes the parameters where they are (float32, bfloat16, float16) and holds its two
-moments in 32 bits or in 8 (1.03 bytes per value and moment, scales included).
+moments in 32 bits or in 8 (1.02 bytes per value and moment, scales included).
 """
 import torch
 

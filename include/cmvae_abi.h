@@ -9,7 +9,8 @@
  *
  * Conventions
  *   - all pointers are DEVICE pointers (HIP, gfx950) unless a name ends in _host;
- *     tensors are dense row-major fp32, labels / indices int64.
+ *     tensors are dense row-major fp32, labels / indices int64 (the descriptors of set
+ *     attention, AdamW and group norm name their types and strides).
  *   - the caller owns every buffer, including `workspace` (size from the matching
  *     *_workspace_bytes query); no entry point allocates, frees or synchronises.
  *   - kernels are enqueued on `stream` (a hipStream_t; NULL = default stream) and the
