@@ -1352,8 +1352,9 @@ static double cost(const Problem& x, const Plan& p) {
 // Four tiles of own rows per workgroup share what they walk; or one tile per workgroup, whose waves share out the walk.  The
 // walk may be cut into pieces, which a second launch joins.
 //   Where four tiles per workgroup fill the card: those, with pieces until there is a workgroup for every slot — twice that for
-//   the causal order at one workgroup per unit (two are dealt in pairs, see place()), and half again as much where lengths will
-//   leave some without work.
+// the causal order at one workgroup per unit (two are dealt in pairs, see place()), half again as much where lengths will leave
+// some without work — or, without lengths, whole, if that costs less (20 x 500 rows x 4 heads of 64 bf16, forward: 18 us whole, 27 in
+// two; 8 x 512 against 2048 rows x 8 heads: 48, 36).
 //   Else whatever costs least of both kinds, whole or in as many pieces as one, two or three turns of the card hold.  Forward +
 //   backward in us, four tiles against one: fp32 4 x 200 rows x 4 heads of 64 67 / 43, 16 x 300 106 / 146, 400 against 8000
 //   141 / 270, causal 4096 x 2 heads of 128 416 / 1261; bf16 32 / 24, 39 / 55, 65 / 78, 160 / 206.
@@ -1365,8 +1366,8 @@ static Plan make_plan(const Problem& x) {
         const int tiles = (x.len + best.tile - 1) / best.tile;
         const long slots = cus * x.occ, want = x.causal && x.occ == 1 ? 2 * slots : x.ragged ? slots + slots / 2 : slots;
         if (wg4 < want && tiles >= 8) {
-            const long ns = (want + wg4 - 1) / wg4;
-            best.nsplit = (int)(ns > tiles / 4 ? tiles / 4 : ns);
+            const Plan p = plan_with(x, 4, (int)std::min((want + wg4 - 1) / wg4, tiles / 4L));
+            if (x.ragged || cost(x, p) < cost(x, best)) best = p;
         }
         return best;
     }
@@ -1427,7 +1428,7 @@ static Sizes sizes_of(const cmvae_set_attn& d) {
     const Problem qside = {es, d.D, nbh, R, d.Sk, false, es * d.D > 256 ? 1 : 2, causal, ragged};
     z.f = R <= most_rows(es, d.D) ? rows_plan(es, d.D, nbh, d.Sk) : make_plan(qside);
     z.q = make_plan(qside);
-    z.k = make_plan({es, d.D, nbh, d.Sk, R, true, es * d.D > 128 ? 1 : 2, causal, ragged});
+    z.k = make_plan({es, d.D, nbh, d.Sk, R, true, d.D == 64 ? 2 : 1, causal, ragged});
     const size_t rows = (size_t)nbh * R, keys = (size_t)nbh * d.Sk;
     z.fwd = z.f.nsplit > 1 ? z.f.nsplit * rows * (d.D + 2) * 4 : 0;
     const size_t bq = z.q.nsplit > 1 ? z.q.nsplit * rows * d.D * 4 : 0;
