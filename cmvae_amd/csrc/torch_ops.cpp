@@ -17,8 +17,10 @@
 
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <cmath>
-#include <unordered_set>
+#include <utility>
+#include <vector>
 
 #include "../../include/cmvae_abi.h"
 
@@ -368,7 +370,15 @@ void adamw_step(at::TensorList params, const c10::List<optional<Tensor>>& grads,
     c10::DeviceGuard guard(exp_avg.device());
     std::vector<cmvae_adamw_tensor> table;
     std::vector<Tensor> keep;
-    std::unordered_set<const void*> seen;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    spans.reserve(params.size() + 3);
+    auto written = [&](const Tensor& t) {
+        const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
+        if (t.numel()) spans.emplace_back(first, first + t.numel() * t.element_size());
+    };
+    written(exp_avg);
+    written(exp_avg_sq);
+    if (given(scales)) written(*scales);
     table.reserve(params.size());
     int64_t at = 0;
     for (size_t i = 0; i < params.size(); ++i) {
@@ -391,9 +401,12 @@ void adamw_step(at::TensorList params, const c10::List<optional<Tensor>>& grads,
             keep.push_back(g);
         }
         if (n == 0) continue;
-        TORCH_CHECK(seen.insert(p.data_ptr()).second, "cmvae_amd adamw: a parameter appears twice");
+        written(p);
         table.push_back({p.data_ptr(), g.data_ptr(), n, here, code});
     }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK(spans[i].first >= spans[i - 1].second, "cmvae_amd adamw: a parameter appears twice, or parameters and states overlap");
     TORCH_CHECK(at == exp_avg.numel(), "cmvae_amd adamw: the parameters take ", at, " state values, the states hold ",
                 exp_avg.numel());
     check(lib.adamw(table.data(), (int)table.size(), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), (float*)ptr(scales),

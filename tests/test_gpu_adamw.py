@@ -325,3 +325,15 @@ def test_more_values_than_32_bits_count(device, bits):
     assert torch.equal(M[at:].view(torch.uint8), m.view(torch.uint8)) and torch.equal(V[at:], v)
     assert sc is None or torch.equal(S[:, at // 256:], sc)
     assert not V[256:at].any()
+
+
+def test_tensors_that_overlap_are_refused(device):
+    from cmvae_amd.optim import adamw_step
+    z = lambda n: torch.zeros(n, device=device)  # noqa: E731
+    buf, g = z(300), z(100)
+    m, v = z(512), z(512)
+    for params, exp_avg, exp_avg_sq in (([buf[:100], buf[99:199]], m, v), ([buf[100:200], buf[:100], buf[150:250]], z(768), z(768)),
+                                        ([buf[:100], z(100)], m, m), ([m[:100], z(100)], m, v), ([z(100), v[412:]], m, v)):
+        with pytest.raises(RuntimeError, match='overlap'):
+            adamw_step(params, [g] * len(params), exp_avg, exp_avg_sq)
+    adamw_step([buf[:100], buf[100:200]], [g, g], m, v)
