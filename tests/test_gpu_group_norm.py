@@ -267,3 +267,23 @@ def test_two_calls_at_once(device):
                 got.append(run(*s, 32, act='elu'))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for a, b in zip(want, got) for x, y in zip(a, b))
+
+
+# rows of which only pairs are aligned, channel pieces of unequal width, groups across thread and piece borders
+MORE = {
+    'pairs': (3, (5, 5), 34, 17),
+    'pairs_in_pieces': (1, (60, 60), 66, 3),
+    'uneven_pieces': (1, (40, 41), 1284, 12),
+    'narrow_pieces': (2, (90, 90), 6, 1),
+    'many_groups': (2, (3, 5), 1152, 576),
+    'more_groups_than_threads': (1, (2, 1), 1536, 1536),
+}
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('case', MORE)
+def test_more_shapes_against_float64(device, case, dtype):
+    N, pix, C, G = MORE[case]
+    x, w, b, dy = make(device, N, pix, C, dtype, seed=6)
+    want, tol, _ = reference(x, w, b, dy, G, 1e-5, 'silu')
+    compare(run(x, w, b, dy, G, act='silu'), want, tol)

@@ -331,3 +331,25 @@ def test_two_calls_at_once(device):
                 got.append(run(*s))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for a, b in zip(want, got) for x, y in zip(a, b))
+
+
+# walks in pieces under both kinds of workgroup, whole walks where four tiles of rows fill the card
+PIECES = {
+    'four_tiles_in_pieces': (1, 300, 2600, 4, 2, 64, False, None, None, True),
+    'four_tiles_in_pieces_causal': (1, 1500, 1500, 2, 1, 128, True, None, None, False),
+    'one_tile_in_pieces': (1, 30, 4100, 4, 4, 64, False, None, [4001], False),
+    'whole': (9, 500, 330, 8, 8, 64, False, None, None, False),
+    'whole_128': (6, 290, 700, 15, 15, 128, True, None, None, True),
+}
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('case', PIECES)
+def test_pieces_against_float64(device, case, dtype):
+    B, Sq, Sk, H, Hkv, D, causal, ql, kl, residual = PIECES[case]
+    q, k, v, do = make(device, B, Sq, Sk, H, Hkv, D, dtype, seed=8)
+    kw = dict(causal=causal, q_len=lens(ql, device), k_len=lens(kl, device), residual=residual)
+    got = run(q, k, v, do, **kw)
+    want, tol = reference(q, k, v, do, 1 / math.sqrt(D), causal, ql, kl, residual)
+    compare(got, want, tol)
+    assert all(torch.equal(x, y) for x, y in zip(got, run(q, k, v, do, **kw)))
