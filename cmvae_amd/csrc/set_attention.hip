@@ -19,7 +19,7 @@
 // bf16 pieces (to nearest, 8 + 8 + 8 bits) and each product as the six piece products that reach above 2^-24 of it —
 // fp32's own accuracy (test_gpu_set_attention.py holds it to fp32 tolerances) at 6/16 of the fp32 instruction's cycles.  An
 // infinite fp32 input makes NaN of its rows.  Scores, softmax statistics, delta and every accumulator are fp32; in the
-// 16-bit types P and dS are rounded once (to nearest) to be factors, dq's dS into two.
+// 16-bit types P and dS are rounded once (to nearest) to be factors, dq's dS into two; fp16's are held times a power of two.
 #include "common.h"
 
 #include <algorithm>
@@ -52,6 +52,8 @@ struct Args {
 // fp16 probabilities are held times 2^15 as factors: p <= 1 fits (32768 < 65504), and a row of many keys, whose p are
 // under fp16's smallest normal 2^-14, keeps 11 bits of each.  The other types have fp32's exponents.
 template <typename T> __device__ constexpr float p_shift() { return std::is_same<T, _Float16>::value ? 15.f : 0.f; }
+// fp16's dS, whose size is that of the gradients, times p, is held times a power of two of its own, see fit_ds(): at first this
+template <typename T> __device__ constexpr float ds_scale() { return std::is_same<T, _Float16>::value ? 0x1p48f : 1.f; }
 
 template <typename T>
 struct Vec8 {};
@@ -208,6 +210,28 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
             if constexpr (LOW && P == 1) acc[d] = mma<T>(a, low, acc[d]);
         }
     }
+}
+
+// fp16: dS as a factor needs a scale.  Unscaled, values under 2^-25 were 0 and those over 65504 infinite — p of 1 / 4096 takes
+// gradients of size 1e-3 to the one end (dq off by 0.5 %), a loss scale takes them to the other.  A lane's column (a query row in
+// dq, a key in dk) holds dS f, f a power of two; where a tile brings a value over 2^15, f, that tile and the sums so far are
+// scaled down until the largest is in [2^12, 2^13) (exactly: f starts at 2^48 and dS f is fp32's until it is rounded).  What is
+// rounded as a subnormal is then 2^26 times smaller than the column's largest value, or under 2^-62.  The lane's other half has the
+// rest of its column; the branch is the wave's, and taken for a column's first tile and a few more.  Forward + backward of 2 x
+// 4096 causal rows x 16 heads of 128 920 -> 996 us, of dense 8 x 4096 x 16 heads of 64 3300 -> 3460; bf16 needs none of it.
+template <int N>
+__device__ __forceinline__ void fit_ds(f32x16& s, f32x16 (&acc)[N], float& f) {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(s[i]));
+    if (__ballot(mx > 0x1p15f) == 0) return;
+    mx = fmaxf(mx, other_half(mx));
+    const int down = mx > 0x1p15f && mx < INFINITY ? (__float_as_int(mx) >> 23) - (127 + 12) : 0;
+    const float by = __int_as_float((127 - down) << 23);
+    s *= by;
+#pragma unroll
+    for (int d = 0; d < N; ++d) acc[d] *= by;
+    f *= by;
 }
 
 // eight channels of a row as fp32
@@ -981,7 +1005,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
     const Frag<T, D> gf = load_frag<T, D>(grow, row_ok, sel);
     const long hrow = ((long)pl.b * a.H + head) * a.Sq + pos;
     const long orow = (((long)pl.b * a.Sq + pos) * a.H + head) * D * es;
-    float dl, lse = INFINITY;
+    float dl, lse = INFINITY, f = ds_scale<T>();
     {
         dl = dot_rows<T, D>(grow, a.att + orow, row_ok);
         if (a.att_low) dl += dot_rows<T, D>(grow, a.att_low + orow, row_ok);
@@ -1009,14 +1033,23 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
             f32x16 s = mul_rows<T, D, KT>(kt, u * 32, qf, zero16());
             f32x16 dp = mul_rows<T, D, KT>(vt, u * 32, gf, zero16());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_raw(fmaf(s[i], a.c, -lse)) * (dp[i] - dl);
+            for (int i = 0; i < 16; ++i) {
+                const float d = std::is_same<T, _Float16>::value ? fmaf(dp[i], f, -dl * f) : dp[i] - dl;      // f: exact
+                s[i] = exp2_raw(fmaf(s[i], a.c, -lse)) * d;
+            }
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (k0 + u * 32 + acc_row(i, h) >= klast) s[i] = 0.f;
             }
+            if constexpr (std::is_same<T, _Float16>::value) fit_ds(s, acc, f);
             mul_cols<T, D, KT, true>(kt, u * 32, s, sel, acc);
         }
+    };
+    auto unscale = [&](f32x16 (&x)[D / 32]) {
+        if constexpr (std::is_same<T, _Float16>::value)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) x[d] *= 1.f / f;
     };
     if constexpr (WS > 1) {
         char* my = smem + w * 2 * TB;
@@ -1030,6 +1063,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
             use(t, my, my + TB);
             wave_sync();
         }
+        unscale(acc);
         hand_over<WS>(smem, w, acc);
         if (w > 0) return;
 #pragma unroll
@@ -1052,6 +1086,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
             }
             __syncthreads();
         }
+        unscale(acc);
     }
     if (r >= a.R) return;
     float* po = a.nsplit > 1 ? a.part + ((long)pl.split * a.B * a.Hkv * a.R + hrow) * D : nullptr;
@@ -1143,6 +1178,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (
         return x;
     };
     constexpr float unshift = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.f;
+    float f = ds_scale<T>();
     typedef Stage<T, D, RT, NW * 64> St;
     St qs, gs;
     const long qss = a.q_ss * es, qsh = a.q_sh * es, gss = a.g_ss * es, gsh = a.g_sh * es;
@@ -1166,7 +1202,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (
                 const int q = one ? 0 : (x.pos + j) / ql;
                 const long at = hrow0 + (long)(x.g + q) * a.Sq + (x.pos + j - q * ql);
                 st_lse = a.lse[at] - p_shift<T>();
-                st_dl = a.delta[at] * unshift;
+                st_dl = a.delta[at];
             }
         }
     };
@@ -1211,10 +1247,19 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (
             for (int q4 = 0; q4 < 4; ++q4) {
                 const f32x4 dl = *reinterpret_cast<const f32x4*>(st + RT + 8 * q4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * q4 + j] *= fmaf(dp[4 * q4 + j], unshift, -dl[j]);
+                for (int j = 0; j < 4; ++j) s[4 * q4 + j] *= dp[4 * q4 + j] - dl[j];
+            }
+            if constexpr (std::is_same<T, _Float16>::value) {
+                s *= f * unshift;                                 // s was p times 2^15
+                fit_ds(s, dk, f);
             }
             mul_cols<T, D, RT>(buf, u * 32, s, sel, dk);
         }
+    };
+    auto unscale = [&](f32x16 (&x)[D / 32]) {
+        if constexpr (std::is_same<T, _Float16>::value)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) x[d] *= 1.f / f;
     };
     if constexpr (WS > 1) {
         char* my = smem + w * BUF;
@@ -1233,6 +1278,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (
             wave_sync();
             x = xn;
         }
+        unscale(dk);
         hand_over<WS>(smem, w, dk);
         if (w == 0)
 #pragma unroll
@@ -1257,6 +1303,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (
             cur ^= 1;
             x = xn;
         }
+        unscale(dk);
     }
     if (key >= a.Sk) return;
     const long krow = ((long)pl.b * a.Sk + key) * a.Hkv + pl.kh;

@@ -353,3 +353,66 @@ def test_pieces_against_float64(device, case, dtype):
     want, tol = reference(q, k, v, do, 1 / math.sqrt(D), causal, ql, kl, residual)
     compare(got, want, tol)
     assert all(torch.equal(x, y) for x, y in zip(got, run(q, k, v, do, **kw)))
+
+
+# walks shared out by waves, of four tiles, in pieces; short and long, so that p and dS are small
+SMALL_DS = {
+    'few_rows': (1, 33, 8000, 2, 1, 64, False, None, None),
+    'one_query': (2, 1, 5000, 4, 2, 128, True, None, [5000, 777]),
+    'long_causal': (1, 1500, 1500, 4, 2, 128, True, None, None),
+    'padded': (4, 500, 2049, 8, 2, 64, False, [500, 129, 1, 0], [2049, 513, 2000, 64]),
+    'whole': (9, 500, 330, 8, 8, 64, False, None, None),
+    'few_keys': (1, 3000, 40, 2, 1, 64, False, None, None),
+}
+
+
+def eighths(do, seed):
+    """Multiples of 1/8 in [-4, 4], none of them 0: exact in fp16 down to 2^-21 times themselves."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(1, 33, do.shape, generator=g) * (1 - 2 * torch.randint(0, 2, do.shape, generator=g))
+    return (x / 8).to(do)
+
+
+@pytest.mark.parametrize('power', [-14, -8, 8])
+@pytest.mark.parametrize('case', SMALL_DS)
+def test_fp16_gradients_are_as_exact_for_small_and_large_do(device, case, power):
+    """The gradients are linear in dO and every step but the results' rounding is the same for dO and 2^power dO, so they are
+    2^power times each other to those roundings: half a step of each result, 2^-11 of it or 2^-25."""
+    B, Sq, Sk, H, Hkv, D, causal, ql, kl = SMALL_DS[case]
+    q, k, v, do = make(device, B, Sq, Sk, H, Hkv, D, 'f16', seed=11)
+    do = eighths(do, 12)
+    kw = dict(causal=causal, q_len=lens(ql, device), k_len=lens(kl, device))
+    f = 2.0 ** power
+    want, got = run(q, k, v, do, **kw), run(q, k, v, (do.float() * f).half(), **kw)
+    assert torch.equal(want[0], got[0])
+    for name, a, b in zip(('dq', 'dk', 'dv'), got[1:], want[1:]):
+        b = b.double() * f
+        assert torch.isfinite(a).all() and torch.isfinite(b).all(), name
+        off = (a.double() - b).abs() - 2.0 ** -10 * (1 + 2.0 ** -10) * b.abs() - 2.0 ** -25 * (1 + f)
+        assert float(off.max()) <= 0, '%s: %.3g over its tolerance' % (name, float(off.max()))
+
+
+def test_fp16_gradients_of_rows_of_unequal_size(device):
+    """Every row of dO times a power of two of its own: dq's rows are its multiples, a small row loses nothing beside a large
+    one."""
+    q, k, v, do = make(device, 1, 200, 3000, 2, 2, 64, 'f16', seed=13)
+    do = eighths(do, 14)
+    f = 2.0 ** torch.randint(-14, 9, (1, 200, 2, 1), generator=torch.Generator().manual_seed(15)).to(device).double()
+    want, got = run(q, k, v, do)[1].double() * f, run(q, k, v, (do.double() * f).half())[1]
+    off = (got.double() - want).abs() - 2.0 ** -10 * (1 + 2.0 ** -10) * want.abs() - 2.0 ** -25 * (1 + f)
+    assert float(off.max()) <= 0
+
+
+@pytest.mark.parametrize('case', [(1, 64, 8, 2, 1, 64), (1, 64, 8, 2, 1, 128), (16, 130, 8, 16, 16, 64)])
+def test_fp16_ds_beyond_its_range(device, case):
+    """dS over 65504 (large values, gradients as a loss scale leaves them) under results that fit."""
+    B, Sq, Sk, H, Hkv, D = case
+    q, k, v, do = make(device, B, Sq, Sk, H, Hkv, D, 'f16', seed=16)
+    q, k, v, do = q * 0.25, k * 0.05, v * 16 + 4 * v.sign(), (do * 1500).clamp(-6900, 6900)
+    heads = lambda t: t.double().repeat_interleave(H // t.shape[2], 2).transpose(1, 2).contiguous()  # noqa: E731
+    p = torch.softmax(heads(q) @ heads(k).transpose(2, 3).contiguous() / math.sqrt(D), -1)
+    dp = heads(do) @ heads(v).transpose(2, 3).contiguous()
+    assert float((p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max()) > 65504
+    want, tol = reference(q, k, v, do, 1 / math.sqrt(D), False, None, None, False)
+    assert all(float(w.abs().max()) < 65504 for w in want)
+    compare(run(q, k, v, do), want, tol)
