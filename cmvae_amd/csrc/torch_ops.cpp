@@ -9,6 +9,7 @@
 // The library's path is handed in by cmvae_amd/_lib.py (`_use_library`), so that CMVAE_HIP_LIB holds here too.  Workspaces
 // come from torch's caching allocator, per call: a captured graph owns its own.
 #include <ATen/ATen.h>
+#include <ATen/TensorUtils.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -80,7 +81,9 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Gradients that cannot be differentiated again say so when that is tried: under create_graph they get a node that throws,
-// between them and what they depend on.
+// between them and what they depend on.  `of` has to hold a tensor that autograd knows for every input that wanted a gradient: a
+// copy made inside of Function::forward is none (grad mode is off there), and with a constant incoming gradient nothing
+// would be left to throw.  So inputs are copied, where they have to be, before Function::apply.
 variable_list once(variable_list grads, const variable_list& of, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
     const size_t n = grads.size();
@@ -125,10 +128,10 @@ cmvae_set_attn describe(const Tensor& q, const Tensor& k, const Tensor& v, const
 
 class SetAttention : public torch::autograd::Function<SetAttention> {
  public:
-    static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, double scale, bool causal,
+    // q, k, v as rows16() leaves them
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal,
                           const optional<Tensor>& q_len, const optional<Tensor>& k_len, bool residual, bool save) {
-        c10::DeviceGuard guard(q0.device());
-        const Tensor q = rows16(q0), k = rows16(k0), v = rows16(v0);
+        c10::DeviceGuard guard(q.device());
         const SetAttentionArgs a = {scale, causal, residual};
         const Tensor o = at::empty(q.sizes(), q.options());
         Tensor attn = o, low, lse;
@@ -216,19 +219,27 @@ Tensor set_attention(const Tensor& q, const Tensor& k, const Tensor& v, double s
                             (*t)->is_contiguous(),
                         "cmvae_amd set_attention: ", n, " must be a dense int32 tensor of shape [", B, "] beside q");
     const bool save = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
-    return SetAttention::apply(q, k, v, scale, causal, q_len, k_len, residual, save);
+    return SetAttention::apply(rows16(q), rows16(k), rows16(v), scale, causal, q_len, k_len, residual, save);
 }
 
 // ------------------------------------------------------------------------------------------------ group norm
-// [N, ..., C] -> [N, P, C] with adjacent channels (a copy where strides do not allow it)
+std::vector<int64_t> sizes3(const Tensor& x) {
+    int64_t P = 1;
+    for (int64_t i = 1; i + 1 < x.dim(); ++i) P *= x.size(i);
+    return {x.size(0), P, x.size(-1)};
+}
+
+// [N, ..., C] as [N, P, C] with adjacent channels (a copy where strides do not allow it)
 Tensor rows3(const Tensor& x) {
-    Tensor r = x;
-    if (x.dim() != 3) {
-        int64_t P = 1;
-        for (int64_t i = 1; i + 1 < x.dim(); ++i) P *= x.size(i);
-        r = x.reshape({x.size(0), P, x.size(-1)});
-    }
+    const Tensor r = x.dim() == 3 ? x : x.reshape(sizes3(x));
     return r.stride(2) == 1 ? r : r.contiguous();
+}
+
+// x, or a dense copy of it where rows3() would make one
+Tensor viewable(const Tensor& x) {
+    if (x.is_contiguous() || (x.dim() == 3 && x.stride(2) == 1)) return x;
+    const auto st = at::detail::computeStride(x.sizes(), x.strides(), sizes3(x));
+    return st && (*st)[2] == 1 ? x : x.contiguous();
 }
 
 void strides2(int64_t (&out)[2], const Tensor& t) {
@@ -250,11 +261,12 @@ cmvae_group_norm describe(const Tensor& x, int64_t groups, const Tensor& w, cons
 
 class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
  public:
+    // x0 as viewable() leaves it, weight and bias dense
     static Tensor forward(AutogradContext* ctx, const Tensor& x0, int64_t groups, const optional<Tensor>& weight,
                           const optional<Tensor>& bias, double eps, int64_t act, bool save) {
         c10::DeviceGuard guard(x0.device());
         const Tensor x = rows3(x0);
-        const Tensor w = given(weight) ? weight->contiguous() : Tensor(), b = given(bias) ? bias->contiguous() : Tensor();
+        const Tensor w = given(weight) ? *weight : Tensor(), b = given(bias) ? *bias : Tensor();
         const Tensor y = at::empty(x0.sizes(), x.options());
         Tensor stats;
         if (save) stats = at::empty({x.size(0), groups, 4}, x.options().dtype(at::kFloat));
@@ -271,19 +283,20 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
             ctx->saved_data["eps"] = eps;
             ctx->saved_data["act"] = act;
             ctx->saved_data["parameters"] = (given(weight) && weight->requires_grad()) || (given(bias) && bias->requires_grad());
-            ctx->save_for_backward({x, w, b, stats});
+            ctx->save_for_backward({x0, w, b, stats});
         }
         return y;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto s = ctx->get_saved_variables();
-        const Tensor &x = s[0], &w = s[1], &b = s[2], &stats = s[3];
+        const Tensor &x0 = s[0], &w = s[1], &b = s[2], &stats = s[3];
         Tensor dx, dw, db;
         {
             at::NoGradGuard no_grad;
-            c10::DeviceGuard guard(x.device());
-            dx = at::empty(g[0].sizes(), x.options());
+            c10::DeviceGuard guard(x0.device());
+            const Tensor x = rows3(x0);
+            dx = at::empty(x0.sizes(), x0.options());
             if (ctx->saved_data["parameters"].toBool()) {
                 if (w.defined()) dw = at::empty(w.sizes(), w.options());
                 if (b.defined()) db = at::empty(b.sizes(), b.options());
@@ -304,7 +317,7 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
                 check(lib.gn_bwd(&d, ptr(ws), n, stream_of(x)), "cmvae_group_norm_bwd");
             }
         }
-        variable_list out = once({dx, dw, db}, {g[0], x, w, b}, "group_norm_act");
+        variable_list out = once({dx, dw, db}, {g[0], x0, w, b}, "group_norm_act");
         return {out[0], Tensor(), out[1], out[2], Tensor(), Tensor(), Tensor()};
     }
 };
@@ -331,7 +344,8 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const optional<Tensor>& w
                 "cmvae_amd group_norm_act: weight and bias are of different types");
     const bool save = at::GradMode::is_enabled() && (x.requires_grad() || (given(weight) && weight->requires_grad()) ||
                                                      (given(bias) && bias->requires_grad()));
-    return GroupNormAct::apply(x, groups, weight, bias, eps, act, save);
+    auto dense = [](const optional<Tensor>& t) { return given(t) ? optional<Tensor>(t->contiguous()) : optional<Tensor>(); };
+    return GroupNormAct::apply(viewable(x), groups, dense(weight), dense(bias), eps, act, save);
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW

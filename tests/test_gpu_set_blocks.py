@@ -234,3 +234,47 @@ def test_command_line_flag(tmp_path):
     assert p.parse_args(base).optimizer == 'adam' and p.parse_args(base + ['--optimizer', 'adamw8']).optimizer == 'adamw8'
     assert subprocess.run([sys.executable, '-m', 'cmvae_amd.main', 'omniglot', *base, '--optimizer', 'sgd'], cwd=ROOT,
                           capture_output=True).returncode != 0
+
+
+def second_derivative_cases(device):
+    """name -> (leaf, call, what the gradient is asked from): inputs that are copied or viewed on the way in, with a gradient of y
+    that is a constant and nothing else that wants one."""
+    from cmvae_amd.attention import set_attention
+    from cmvae_amd.norm import group_norm_act
+    leaf = lambda *s: torch.randn(*s, device=device, requires_grad=True)  # noqa: E731
+    nchw, image, pixel, flat = leaf(2, 8, 3, 3), leaf(2, 3, 3, 8), leaf(5, 8), leaf(2 * 4 * 2 * 64 + 1)
+    tall, thin = leaf(2, 6, 3, 8), leaf(2, 3, 3, 8)
+    wide, frozen, scale = leaf(2, 4, 2, 128), torch.ones(8, device=device), leaf(16)
+    q, k, v = torch.randn(3, 2, 4, 2, 64, device=device)
+    row = flat[1:].view(2, 4, 2, 64)                            # rows that do not start at multiples of 16 bytes
+    col = wide[..., ::2]                                        # channels that are not adjacent
+    x = torch.randn(2, 3, 3, 8, device=device)
+    return {
+        'channels first': (nchw, lambda: group_norm_act(nchw.permute(0, 2, 3, 1), 2)),
+        'channels first, frozen parameters': (nchw, lambda: group_norm_act(nchw.permute(0, 2, 3, 1), 2, frozen, frozen, act='silu')),
+        'an image': (image, lambda: group_norm_act(image, 2, act='elu')),
+        'one pixel': (pixel, lambda: group_norm_act(pixel, 2)),
+        'every other image row': (tall, lambda: group_norm_act(tall[:, ::2], 2)),
+        'one channel': (thin, lambda: group_norm_act(thin[..., :1], 1, act='silu')),
+        'strided parameters': (scale, lambda: group_norm_act(x, 2, scale[::2], act='silu')),
+        'misaligned q': (flat, lambda: set_attention(row, k, v)),
+        'misaligned k': (flat, lambda: set_attention(q, row, v)),
+        'strided v': (wide, lambda: set_attention(q, k, col)),
+        'all copied': (wide, lambda: set_attention(col, col, col)),
+    }
+
+
+@pytest.mark.parametrize('name', ['channels first', 'channels first, frozen parameters', 'an image', 'one pixel',
+                                  'every other image row', 'one channel', 'strided parameters', 'misaligned q', 'misaligned k', 'strided v', 'all copied'])
+def test_second_derivatives_of_copied_inputs_say_so(device, name):
+    """The same where the kernels read a copy or a view of the input and dO is a constant: without its refusal a penalty on the gradient
+    would be dropped.  A gradient under create_graph that is not differentiated is the plain one."""
+    leaf, call = second_derivative_cases(device)[name]
+    d = torch.randn_like(call())
+    (plain,) = torch.autograd.grad(call(), leaf, d)
+    (g,) = torch.autograd.grad(call(), leaf, d, create_graph=True)
+    assert g.requires_grad and torch.equal(g, plain)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        g.square().sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        torch.autograd.grad(g.square().sum(), leaf, allow_unused=True)
