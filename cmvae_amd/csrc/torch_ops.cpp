@@ -384,11 +384,16 @@ void adamw_step(at::TensorList params, const c10::List<optional<Tensor>>& grads,
     c10::DeviceGuard guard(exp_avg.device());
     std::vector<cmvae_adamw_tensor> table;
     std::vector<Tensor> keep;
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    // what the launch writes, and what it reads only: a workgroup may read before or after another one writes
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans, reads;
     spans.reserve(params.size() + 3);
-    auto written = [&](const Tensor& t) {
+    reads.reserve(params.size() + 1);
+    auto span = [](const Tensor& t) {
         const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
-        if (t.numel()) spans.emplace_back(first, first + t.numel() * t.element_size());
+        return std::make_pair(first, first + t.numel() * t.element_size());
+    };
+    auto written = [&](const Tensor& t) {
+        if (t.numel()) spans.push_back(span(t));
     };
     written(exp_avg);
     written(exp_avg_sq);
@@ -416,11 +421,18 @@ void adamw_step(at::TensorList params, const c10::List<optional<Tensor>>& grads,
         }
         if (n == 0) continue;
         written(p);
+        if (g.data_ptr() != p.data_ptr()) reads.push_back(span(g));       // its own parameter: one thread reads both, then writes
         table.push_back({p.data_ptr(), g.data_ptr(), n, here, code});
     }
+    if (given(step_dev)) reads.push_back(span(*step_dev));
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
         TORCH_CHECK(spans[i].first >= spans[i - 1].second, "cmvae_amd adamw: a parameter appears twice, or parameters and states overlap");
+    for (const auto& r : reads) {
+        const auto after = std::lower_bound(spans.begin(), spans.end(), std::make_pair(r.second, uintptr_t(0)));
+        TORCH_CHECK(after == spans.begin() || std::prev(after)->second <= r.first,
+                    "cmvae_amd adamw: a gradient or the step count overlaps a parameter or a state that the step writes");
+    }
     TORCH_CHECK(at == exp_avg.numel(), "cmvae_amd adamw: the parameters take ", at, " state values, the states hold ",
                 exp_avg.numel());
     check(lib.adamw(table.data(), (int)table.size(), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), (float*)ptr(scales),

@@ -23,8 +23,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, scales=None, step=1, lr=1e-3,
     """One AdamW step, in place, over the tensors `params` with gradients `grads` (None: the tensor and its states are left
     as they are).
 
-    params: dense float32 / bfloat16 / float16 tensors that overlap neither each other nor the states (types may be
-    mixed; a gradient has its parameter's).
+    params: dense float32 / bfloat16 / float16 tensors that overlap neither each other nor the states nor what is read: other
+    tensors' gradients, `step` (types may be mixed; a gradient has its parameter's).
     exp_avg, exp_avg_sq: the flat states of all tensors in order, each padded to a multiple of 256 values in the order of
     its parameter's memory (`state_size`); float32, or float8_e4m3fn and uint8 with `scales` [2, length / 256].
     step: 1, 2, ...; or an int64 tensor of one value on the device (for a step replayed from a HIP graph).

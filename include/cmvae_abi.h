@@ -345,7 +345,8 @@ int cmvae_adam_step_dev(float* param, const float* grad, float* exp_avg, float* 
 /* ==== AdamW (decoupled weight decay) over many tensors, with states in 32 or in 8 bits:
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
  * tensors_host: `count` descriptors in HOST memory, read before the call returns (the kernels get them as launch arguments);
- * param and grad are dense, of one dtype (CMVAE_F32 / BF16 / F16), no two tensors overlap.  exp_avg, exp_avg_sq: flat, the
+ * param and grad are dense, of one dtype (CMVAE_F32 / BF16 / F16); what is written (params, states, scales) overlaps neither
+ * itself nor a grad (but a grad may be its own param) nor step_dev.  exp_avg, exp_avg_sq: flat, the
  * states of a tensor start at `state` (a multiple of 256) and take its n values rounded up to a multiple of 256.
  * state_bits 32: fp32.  8: one byte per value, scales [2][state_len / 256] fp32 (first moment's, then second's); exp_avg is
  * e4m3 of m / scale, exp_avg_sq = c stands for scale * 2^((c >> 3) - 31) * (1 + (c & 7) / 8), 0 for 0, 255 for a value that

@@ -337,3 +337,38 @@ def test_tensors_that_overlap_are_refused(device):
         with pytest.raises(RuntimeError, match='overlap'):
             adamw_step(params, [g] * len(params), exp_avg, exp_avg_sq)
     adamw_step([buf[:100], buf[100:200]], [g, g], m, v)
+
+
+def test_what_is_read_overlaps_nothing_that_is_written(device):
+    """A gradient inside of another stepped parameter, of a state, or shifted against its own parameter, and a step count inside
+    of a state would be read before or after they are written, as it happens: refused.  Nothing is launched."""
+    from cmvae_amd.optim import adamw_step
+    z = lambda n, dt=torch.float32: torch.zeros(n, device=device, dtype=dt)  # noqa: E731
+    m, v, p, g, buf = z(10240), z(10240), z(5000), z(5000), z(5001)
+    for params, grads, step in (([p, g], [g, z(5000)], 1), ([p, g], [z(5000), p], 1), ([buf[:5000], p], [buf[1:], g], 1),
+                                ([buf[1:], p], [buf[:5000], g], 1), ([p, z(5000)], [g, m[5120:10120]], 1),
+                                ([p, z(5000)], [v[:5000], g], 1), ([p, z(5000)], [g, z(5000)], m.view(torch.int64)[7:8])):
+        with pytest.raises(RuntimeError, match='overlap'):
+            adamw_step(params, grads, m, v, step=step)
+    m8, v8, scales = z(10496, torch.uint8).view(torch.float8_e4m3fn), z(10496, torch.uint8), z(82).view(2, 41)
+    with pytest.raises(RuntimeError, match='overlap'):
+        adamw_step([z(10160), z(80)], [z(10160), scales.view(-1)[1:81]], m8, v8, scales)
+    assert not any(t.any() for t in (m, v, p, g, buf, scales))
+
+
+def test_gradients_that_may_share_memory(device):
+    """One gradient of several parameters, a parameter that is left out, neighbours in one buffer, a parameter as its own gradient."""
+    from cmvae_amd.optim import adamw_step
+    g = torch.Generator().manual_seed(8)
+    flat = torch.randn(4 * 5000, generator=g).to(device)
+    p0, g0, p1, g1 = flat.view(4, 5000).unbind(0)
+    for ps, gs in (([p0, p1], [g0, g1]), ([p0, p1], [g0, g0]), ([p0, g1], [p1, None]), ([p0, p1], [p0, g1])):
+        m, v = torch.zeros(10240, device=device), torch.zeros(10240, device=device)
+        want, _, _, _ = reference(ps, [torch.zeros_like(p) if x is None else x for p, x in zip(ps, gs)], m, v, None, 1, **HYPER)
+        old = g1.clone()
+        adamw_step(ps, gs, m, v, step=1, **HYPER)
+        for p, x, (w, tol) in zip(ps, gs, want):
+            if x is None:
+                assert torch.equal(p, old)
+            else:
+                within(p, w, tol, 'p')
