@@ -6,13 +6,14 @@
 //   dx = rstd (dz w_c - m1 - xhat m2),   m1, m2 = means over the group of dz w_c and dz w_c xhat
 //
 // Both directions are bound by memory.  A sample whose rows fit in the registers of one workgroup is read once and written
-// once (resident kernels; 800 x 196 x 64 fp32: 22 us forward, 30 backward, 3.6 and 4.0 TB/s); a larger one takes a pass for its
+// once (resident kernels; 800 x 196 x 64 fp32: 23 us forward, 30 backward, 3.5 and 4.0 TB/s); a larger one takes a pass for its
 // sums, a small launch that finishes them, and a pass that applies them (16 x 9216 x 320 bf16: 64 us forward, 108 backward, 4.4
 // TB/s over what the passes move).  A thread's sums are per channel, so a group may end anywhere in its vector.
 //
-// The forward's sums of x and x^2 are fp64 (full rate on this card, and two instructions of the few per value): no
-// shift, no second pass, and a variance that survives a mean thousands of deviations away.  The mean is kept as two fp32
-// numbers for the same reason.  The backward's sums are of mixed sign and fp32 in a thread, fp64 where threads meet.
+// The forward's sums are of d and d^2 in fp64, d = x - (the group's first value): no second pass, and what the variance loses to
+// the mean is 2^-53 of the square of a difference, not of a value.  (Sums of x and x^2 leave 2^-52 x^2 where a group holds
+// one value: at x = 10^5 more than eps, and rstd a third of what it is.  The difference costs the resident forward 4 %.)  The mean is kept as two fp32 numbers for the same
+// reason.  The backward's sums are of mixed sign and fp32 in a thread, fp64 where threads meet.
 // Sums are added in a fixed order: every run gives the same bits.
 #include "common.h"
 
@@ -30,7 +31,7 @@ struct Args {
     float2* bpart;                              // backward sums [N, pc, C]
     float2* means;                              // m1, m2 [N, G]
     long x_sn, x_sp, g_sn, g_sp;                // strides in elements
-    int N, P, C, G, Cg, CV, act, wtype;
+    int N, P, C, G, Cg, CV, act, wtype, xtype;
     int pc, rows_per, cc, cw;                   // pixel pieces per sample, pixels per piece, channel pieces, vectors per one
     float eps;
 };
@@ -65,12 +66,12 @@ __device__ __forceinline__ typename Vec<T, V>::type pack(const float (&x)[V]) {
     return p;
 }
 
-__device__ __forceinline__ float param(const void* p, int type, int c, float none) {
-    if (!p) return none;
+__device__ __forceinline__ float value(const void* p, int type, long c) {
     if (type == CMVAE_F32) return ((const float*)p)[c];
     if (type == CMVAE_BF16) return (float)((const __bf16*)p)[c];
     return (float)((const _Float16*)p)[c];
 }
+__device__ __forceinline__ float param(const void* p, int type, int c, float none) { return p ? value(p, type, c) : none; }
 __device__ __forceinline__ void put_param(void* p, int type, int c, double v) {
     if (!p) return;
     if (type == CMVAE_F32) ((float*)p)[c] = (float)v;
@@ -113,8 +114,9 @@ __device__ __forceinline__ void slope(const float (&z)[V], float (&d)[V], int ac
     }
 }
 
-__device__ __forceinline__ float4 make_stats(double s1, double s2, double m, float eps) {
-    const double mean = s1 / m, var = fmax(s2 / m - mean * mean, 0.0);
+// from the sums of d = x - first and d^2 over m values
+__device__ __forceinline__ float4 make_stats(double s1, double s2, float first, double m, float eps) {
+    const double off = s1 / m, var = fmax(s2 / m - off * off, 0.0), mean = (double)first + off;
     const float hi = (float)mean;
     return make_float4(hi, (float)(mean - (double)hi), (float)(1.0 / sqrt(var + (double)eps)), 0.f);
 }
@@ -138,6 +140,22 @@ __device__ __forceinline__ void load_stats(const Args& a, const float4* st, int 
     for (int j = 0; j < V; ++j) {
         const float4 s = st[(c0 + j) / a.Cg];
         k.mh[j] = s.x; k.ml[j] = s.y; k.rs[j] = s.z;
+    }
+}
+
+// the first value of each of a thread's channels' groups; x: the sample
+template <typename T, int V>
+__device__ __forceinline__ void load_first(const Args& a, const T* x, int c0, double (&first)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) first[j] = (double)(float)x[(c0 + j) / a.Cg * a.Cg];
+}
+template <int V>
+__device__ __forceinline__ void add_to(const float (&v)[V], const double (&first)[V], double (&s1)[V], double (&s2)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const double d = (double)v[j] - first[j];
+        s1[j] += d;
+        s2[j] = fma(d, d, s2[j]);
     }
 }
 
@@ -221,9 +239,11 @@ __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
     const bool on = t < A;
     const T* x = (const T*)a.x + n * a.x_sn + c0;
     TV hold[R];
-    double s1[V], s2[V];
+    double first[V], s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
+    if (on) load_first<T, V>(a, x - c0, c0, first);
+    for (int g = t; g < a.G; g += THREADS) st[g].x = (float)(x - c0)[g * a.Cg];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int p = row + i * rows;
@@ -234,12 +254,7 @@ __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
         if (on && row + i * rows < a.P) {
             float v[V];
             unpack<T, V>(hold[i], v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double d = (double)v[j];
-                s1[j] += d;
-                s2[j] = fma(d, d, s2[j]);
-            }
+            add_to<V>(v, first, s1, s2);
         }
     }
     if (one) {
@@ -259,7 +274,7 @@ __global__ __launch_bounds__(THREADS) void fwd_resident_kernel(Args a) {
         const int r = i / w;
         return red[r * pitch + g * w + i - r * w];
     }, [&](int g, double2 u) {
-        const float4 q = make_stats(u.x, u.y, (double)a.P * a.Cg, a.eps);
+        const float4 q = make_stats(u.x, u.y, st[g].x, (double)a.P * a.Cg, a.eps);
         st[g] = q;
         if (a.stats) a.stats[(long)n * a.G + g] = q;
     });
@@ -400,18 +415,16 @@ __global__ __launch_bounds__(256) void fwd_sums_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0;
     const T* x = (const T*)a.x + q.n * a.x_sn + q.c0;
-    if (q.on)
+    if (q.on) {
+        double first[V];
+        load_first<T, V>(a, x - q.c0, q.c0, first);
 #pragma unroll 4
         for (int p = q.p0 + q.row; p < q.p1; p += q.rows) {
             float v[V];
             unpack<T, V>(*reinterpret_cast<const TV*>(x + p * a.x_sp), v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double d = (double)v[j];
-                s1[j] += d;
-                s2[j] = fma(d, d, s2[j]);
-            }
+            add_to<V>(v, first, s1, s2);
         }
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) red[threadIdx.x * V + j] = make_double2(s1[j], s2[j]);
     __syncthreads();
@@ -448,8 +461,9 @@ template <int FIN>
 __global__ __launch_bounds__(FIN) void fwd_finish_kernel(Args a) {
     const long ng = blockIdx.x;
     const int n = (int)(ng / a.G), g = (int)(ng - (long)n * a.G);
+    const float first = value(a.x, a.xtype, n * a.x_sn + g * a.Cg);
     const double2 s = block_sum<FIN>(a.part + (long)n * a.pc * a.C + g * a.Cg, a.pc, a.C, a.Cg, [](int) { return 1.0; });
-    if (threadIdx.x == 0) a.stats[ng] = make_stats(s.x, s.y, (double)a.P * a.Cg, a.eps);
+    if (threadIdx.x == 0) a.stats[ng] = make_stats(s.x, s.y, first, (double)a.P * a.Cg, a.eps);
 }
 
 template <typename T, int V>
@@ -718,7 +732,7 @@ static Args args_of(const cmvae_group_norm& d, const Plan& p, int V) {
     a.x_sn = d.x_stride[0]; a.x_sp = d.x_stride[1];
     a.g_sn = d.dy_stride[0]; a.g_sp = d.dy_stride[1];
     a.N = d.N; a.P = d.P; a.C = d.C; a.G = d.G; a.Cg = d.C / d.G; a.CV = d.C / V;
-    a.act = d.act; a.wtype = d.wdtype; a.eps = d.eps;
+    a.act = d.act; a.wtype = d.wdtype; a.xtype = d.dtype; a.eps = d.eps;
     a.pc = p.pc; a.rows_per = p.rows_per; a.cc = p.cc; a.cw = p.cw;
     return a;
 }

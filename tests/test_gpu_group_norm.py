@@ -287,3 +287,26 @@ def test_more_shapes_against_float64(device, case, dtype):
     x, w, b, dy = make(device, N, pix, C, dtype, seed=6)
     want, tol, _ = reference(x, w, b, dy, G, 1e-5, 'silu')
     compare(run(x, w, b, dy, G, act='silu'), want, tol)
+
+
+@pytest.mark.parametrize('value', [1000.1, 100000.1, 1234567.1])
+@pytest.mark.parametrize('case', ['wave', 'middle', 'large_resident', 'odd_channels', 'split_groups', 'long'])
+def test_groups_of_one_value_far_from_zero(device, case, value):
+    """A group that holds one value has no variance, however large the value: rstd is that of eps.  So it is beside a
+    sample whose values lie one apart around it."""
+    N, pix, C, G = CASES[case]
+    x, w, b, dy = make(device, N, pix, C, 'f32', seed=2)
+    x = x.round() + value
+    x[0] = value
+    want, tol, _ = reference(x, w, b, dy, G, 1e-5, 'silu')
+    compare(run(x, w, b, dy, G, act='silu'), want, tol)
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+def test_groups_of_one_value_in_16_bits(device, dtype):
+    for case in ('middle', 'split_groups'):
+        N, pix, C, G = CASES[case]
+        x, w, b, dy = make(device, N, pix, C, dtype)
+        x[0] = 50000.0
+        want, tol, _ = reference(x, w, b, dy, G, 1e-5, None)
+        compare(run(x, w, b, dy, G), want, tol)
