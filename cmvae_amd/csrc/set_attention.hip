@@ -19,7 +19,7 @@
 // bf16 pieces (to nearest, 8 + 8 + 8 bits) and each product as the six piece products that reach above 2^-24 of it —
 // fp32's own accuracy (test_gpu_set_attention.py holds it to fp32 tolerances) at 6/16 of the fp32 instruction's cycles.  An
 // infinite fp32 input makes NaN of its rows.  Scores, softmax statistics, delta and every accumulator are fp32; in the
-// 16-bit types P and dS are rounded once (to nearest) to be factors, dq's dS into two; fp16's are held times a power of two.
+// 16-bit types P and dS are factors in two parts, each to nearest; fp16's are held times a power of two.
 #include "common.h"
 
 #include <algorithm>
@@ -167,11 +167,13 @@ __device__ __forceinline__ f32x16 mul_rows(const char* tile, int row0, const Fra
 // Register r of the accumulator is tile row acc_row(r, h), which fixes the contraction's order: registers 8s .. 8s + 7 are
 // one instruction's eight; the matching first factor — four rows at one channel, twice — comes from the transposing LDS
 // read (16 lanes name 4 rows x 16 channels, lane i receives channel i of the four rows).
-//   LOW (16-bit types): what the accumulator's rounding leaves is a factor of its own.  dq takes it: a row's sum over dS k
-// cancels what the keys have in common, the roundings of dS do not, and dq's error was 1.52 times that of its own rounding —
-// 1.06 with it, for a third more matrix instructions (dq of dense 8 x 4096 x 16 heads of 64 bf16 1018 -> 1142 us).  dk and dv, summed
-// over many queries, are at 1.4 without.
-template <typename T, int D, int ROWS, bool LOW = false>
+//   16-bit types: the accumulator is a factor twice, as its rounding and as what that leaves.  Every result's error (2-norm,
+// against float64) is then that of its own rounding, to three digits; with one factor o's was 1.16 to 1.31 times that, dq's 1.5 and
+// dk's and dv's 1.42.  One factor (two for dq alone) against two, us: forward + backward of 2 x 4096 causal rows x 16 heads of 128 bf16
+// 870 / 1005, of 8 x 777 against 2049 x 8 heads of 64 fp16 168 / 190; forward of one token x 32 heads of 128 against 16 lists of up
+// to 8191 75.5 / 78.5; dense 8 x 4096 x 16 heads bf16, forward 805 / 1060 (heads of 64) and 1524 / 1790 (128), dk dv 1500 / 1990 and
+// 3720 / 4500.
+template <typename T, int D, int ROWS>
 __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, const Sel& sel, f32x16 (&acc)[D / 32]) {
     constexpr int P = Elem<T>::P;
     typedef __attribute__((address_space(3))) s16x4 lds4;
@@ -190,11 +192,9 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = (T)w[8 * s + j];
             b[0] = __builtin_bit_cast(u32x4, v);
-            if constexpr (LOW) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (T)(w[8 * s + j] - (float)v[j]);
-                low[0] = __builtin_bit_cast(u32x4, v);
-            }
+            for (int j = 0; j < 8; ++j) v[j] = (T)(w[8 * s + j] - (float)v[j]);
+            low[0] = __builtin_bit_cast(u32x4, v);
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
@@ -207,7 +207,7 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
                 a[k] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
             acc[d] = mma<T>(a, b, acc[d]);
-            if constexpr (LOW && P == 1) acc[d] = mma<T>(a, low, acc[d]);
+            if constexpr (P == 1) acc[d] = mma<T>(a, low, acc[d]);
         }
     }
 }
@@ -218,7 +218,8 @@ __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x1
 // scaled down until the largest is in [2^12, 2^13) (exactly: f starts at 2^48 and dS f is fp32's until it is rounded).  What is
 // rounded as a subnormal is then 2^26 times smaller than the column's largest value, or under 2^-62.  The lane's other half has the
 // rest of its column; the branch is the wave's, and taken for a column's first tile and a few more.  Forward + backward of 2 x
-// 4096 causal rows x 16 heads of 128 920 -> 996 us, of dense 8 x 4096 x 16 heads of 64 3300 -> 3460; bf16 needs none of it.
+// 4096 causal rows x 16 heads of 128 920 -> 996 us, of dense 8 x 4096 x 16 heads of 64 3300 -> 3460; bf16 needs none of it
+// (both before the factors' second parts).
 template <int N>
 __device__ __forceinline__ void fit_ds(f32x16& s, f32x16 (&acc)[N], float& f) {
     float mx = 0.f;
@@ -314,7 +315,7 @@ __device__ __forceinline__ f32x4 load4(const char* p) {
 }
 
 // one piece of a result row: o without the residual (16-bit types: and what its rounding leaves, so that the backward's delta is
-// not that of a rounded o — dk's error is then 1.43 times its own rounding's, not 1.47, and dq's 1.06, not 1.19), and o
+// not that of a rounded o, which would leave dq's error at 1.07 to 1.11 times its own rounding's and dk's at up to 1.05), and o
 template <typename T>
 __device__ __forceinline__ void store_o(const Args& a, long at, const char* residual, f32x4 o) {
     if (a.ocopy) store4<T>(a.ocopy + at, o[0], o[1], o[2], o[3]);
@@ -525,8 +526,8 @@ __device__ __forceinline__ void take_over(const char* smem, int w, float f, f32x
 // Keys in tiles of KT through LDS.  Running maximum m (log2 units) and sum l per row.  nsplit > 1: a workgroup covers one
 // piece of the tiles and leaves (acc, m, l) for the joining kernel.
 //   Bound by the matrix instructions and, between them, the exponentials and the LDS reads that feed them: with two workgroups
-// per unit one computes while the other waits.  Dense 8 x 4096 x 16 heads, bf16: 700 TFLOP/s with 64 channels, 750 with 128 (a
-// large library product reaches 1130); fp32 (six bf16 products each), 8 x 2048 x 8 heads: 173 and 150 (the library's fp32
+// per unit one computes while the other waits.  Dense 8 x 4096 x 16 heads, bf16: 520 TFLOP/s with 64 channels, 610 with 128 (a
+// large library product reaches 1130), P's second part, half as much again, not counted; fp32 (six bf16 products each), 8 x 2048 x 8 heads: 173 and 150 (the library's fp32
 // product 153).
 template <typename T, int D, int NW, int KT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
@@ -722,10 +723,13 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float dot2(unsigned a, unsigned b, float c, _Float16) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
 }
+// two values as their roundings and as what those leave
 template <typename T>
-__device__ __forceinline__ unsigned pack2(float x, float y) {
+__device__ __forceinline__ void split2(float x, float y, unsigned (&p)[2]) {
     typedef T T2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x, y}, T2));
+    const T2 a = __builtin_convertvector(f32x2{x, y}, T2);
+    p[0] = __builtin_bit_cast(unsigned, a);
+    p[1] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x - (float)a[0], y - (float)a[1]}, T2));
 }
 
 template <typename T, int D, int R>
@@ -823,9 +827,10 @@ __global__ __launch_bounds__(256) void fwd_rows_kernel(Args a) {
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const unsigned pp = pack2<T>(p[r][u], p[r][u + 1]);
+                    unsigned pp[2];                                 // as in mul_cols(): p's rounding and what that leaves
+                    split2<T>(p[r][u], p[r][u + 1], pp);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[r][e] = dot2(pp, y[e], acc[r][e], T());
+                    for (int e = 0; e < 8; ++e) acc[r][e] = dot2(pp[0], y[e], dot2(pp[1], y[e], acc[r][e], T()), T());
                 }
             }
         }
@@ -969,7 +974,7 @@ __device__ __forceinline__ bool join_sum(const Args& a, const float* part, long 
 
 // ------------------------------------------------------------------------------------------------ backward, query side
 // The forward's shape; delta_i from the saved o, kept for the key side.  Bound as the forward; at its dense sizes, counting three
-// products, bf16 720 TFLOP/s with 64 channels and 740 with 128 (its fourth product, of what dS's rounding leaves, not counted),
+// products, bf16 670 TFLOP/s with 64 channels and 710 with 128 (a fourth, of what dS's rounding leaves, not counted),
 // fp32 203 and 175.
 template <typename T, int D, int NW, int KT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void dq_kernel(Args a) {
@@ -1043,7 +1048,7 @@ __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 :
                     if (k0 + u * 32 + acc_row(i, h) >= klast) s[i] = 0.f;
             }
             if constexpr (std::is_same<T, _Float16>::value) fit_ds(s, acc, f);
-            mul_cols<T, D, KT, true>(kt, u * 32, s, sel, acc);
+            mul_cols<T, D, KT>(kt, u * 32, s, sel, acc);
         }
     };
     auto unscale = [&](f32x16 (&x)[D / 32]) {
@@ -1128,9 +1133,10 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------ backward, key side
 // 32 keys per wave; query rows of the key head's list in tiles of RT through LDS, with their lse and delta.  Bound as the
 // others, and with 128 channels by its registers: 128 accumulators and 128 of fragments leave one wave per SIMD, which waits out
-// its LDS reads itself (bf16, dense 8 x 4096 x 16 heads: 800 TFLOP/s with 64 channels, 600 with 128; fp32, 8 x 2048 x 8: 205 and
-// 170).  Not faster there: fragments requested a step ahead (600 -> 618, but 64 channels lose as much), tiles without padding in
-// a swizzled order (a third fewer bank conflicts, same time), dk and dv in workgroups of their own (548).
+// its LDS reads itself (bf16, dense 8 x 4096 x 16 heads, four products counted of six: 550 TFLOP/s with 64 channels, 490 with 128;
+// fp32, 8 x 2048 x 8: 205 and 170).  Not faster with 128 channels, when four products were all and took 600 TFLOP/s: fragments
+// requested a step ahead (618, but 64 channels lose as much), tiles without padding in a swizzled order (a third fewer bank
+// conflicts, same time), dk and dv in workgroups of their own (548).
 template <typename T, int D, int NW, int RT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && (sizeof(T) * D <= 128 || (sizeof(T) == 4 && D == 64)) ? 2 : 1) void dkv_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -1439,8 +1445,8 @@ static Plan make_plan(const Problem& x) {
 }
 
 // Rows per key head up to which fwd_rows_kernel takes a list: its arithmetic grows with the rows, the matrix instructions' does
-// not.  Rows kernel / the other, us, for 16 lists of 8191 keys x 8 heads: bf16 heads of 128, 1 row 102 / 103, 2 103 / 102, 4 112 /
-// 105, 8 156 / 103; fp32 heads of 64, 4 rows 108 / 107 and for 16 of 2000 30 / 34 (6 rows 58 / 35); fp32 heads of 128, 1 row 193 /
+// not.  Rows kernel / the other, us, for 16 lists of 8191 keys x 8 heads: bf16 heads of 128, 1 row 99 / 102, 2 102 / 104, 4 110 /
+// 101, 8 167 / 105; fp16 heads of 64 50 / 51, 51 / 50, 55 / 50, 102 / 51; fp32 heads of 64, 4 rows 108 / 107 and for 16 of 2000 30 / 34 (6 rows 58 / 35); fp32 heads of 128, 1 row 193 /
 // 332, 8 262 / 330; one list of 8192 keys x 8 heads of 128, 1 row, bf16 10 / 14.
 constexpr int most_rows(int esize, int D) { return esize == 2 ? 2 : D == 64 ? 4 : 8; }
 

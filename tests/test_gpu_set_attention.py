@@ -416,3 +416,54 @@ def test_fp16_ds_beyond_its_range(device, case):
     want, tol = reference(q, k, v, do, 1 / math.sqrt(D), False, None, None, False)
     assert all(float(w.abs().max()) < 65504 for w in want)
     compare(run(q, k, v, do), want, tol)
+
+
+def bounds(q, k, v, do, scale, causal):
+    """(o, dq, dk, dv) in float64 and what each may be off by BEFORE its own rounding: reference()'s terms without lengths, with
+    factors held to f = r^2 (two parts of the element type), o's low part kept for delta (r^2, or half fp16's smallest step) and fp16's
+    dS held until its column's largest is over 2^12."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1:3]
+    u, r = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
+    f, half = r * r, q.dtype == torch.float16
+    zp, zd, zo = (2.0 ** -40, 2.0 ** -37, 2.0 ** -25) if half else (2.0 ** -126, 0.0, 0.0)
+    heads = lambda t: t.double().repeat_interleave(H // t.shape[2], 2).transpose(1, 2).contiguous()  # noqa: E731
+    Q, K, V, G = (heads(t) for t in (q, k, v, do))
+    T = lambda t: t.transpose(2, 3).contiguous()  # noqa: E731
+    s = scale * Q @ T(K)
+    if causal:
+        s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1 + Sk - Sq), -math.inf)
+    p = torch.softmax(s, -1)
+    e = u * ((D + 6) * float((scale * Q.abs() @ T(K.abs())).max()) + math.log(Sk) + 8)
+    ep = 2 * e + (Sk + 4) * u
+    o = p @ V
+    to = (ep + f + (Sk + 4) * u) * (p @ V.abs()) + zp * V.abs().sum(2, keepdim=True)
+    dp, adp = G @ T(V), G.abs() @ T(V.abs())
+    ds = p * (dp - (G * o).sum(-1, keepdim=True))
+    edl = (G.abs() * (to + (r * r + D * u) * o.abs() + zo)).sum(-1, keepdim=True)
+    eds = p * (1 + ep) * ((D + 2) * u * adp + edl) + (ep + f + 4 * u) * ds.abs() + 2.0 ** -126 * adp
+    row, col = (eds + zd * ds.abs().amax(i, keepdim=True) for i in (3, 2))
+    n = Sq * H // Hkv
+    tq = scale * (row + (Sk + 5) * u * ds.abs()) @ K.abs()
+    tk = scale * T(col + (n + 6) * u * ds.abs()) @ Q.abs()
+    tv = T((ep + f + (n + 6) * u) * p + zp) @ G.abs()
+    back = lambda t: t.transpose(1, 2)  # noqa: E731
+    sums = lambda t: back(t).unflatten(2, (Hkv, H // Hkv)).sum(3)  # noqa: E731
+    return [back(o), back(scale * ds @ K), sums(scale * T(ds) @ Q), sums(T(p) @ G)], [back(to), back(tq), sums(tk), sums(tv)]
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('case', [(2, 1, 700, 2, 2, 64, False), (2, 1, 600, 4, 2, 128, True), (1, 1, 500, 8, 2, 64, False),
+                                  (2, 150, 150, 4, 2, 64, True), (2, 90, 210, 2, 1, 128, False), (16, 130, 140, 16, 16, 64, True),
+                                  (16, 130, 100, 16, 8, 128, False)])
+def test_16_bit_results_are_off_by_their_own_rounding(device, case, dtype):
+    """p and dS as factors, and the o that delta is of, hold twice the type's bits: a result is within half a step of float64's and
+    the little that is left of fp32's sums and of those factors."""
+    B, Sq, Sk, H, Hkv, D, causal = case
+    q, k, v, do = make(device, B, Sq, Sk, H, Hkv, D, dtype, seed=21)
+    r, tiny = torch.finfo(q.dtype).eps / 2, float(torch.finfo(q.dtype).smallest_normal)
+    want, tol = bounds(q, k, v, do, 1 / math.sqrt(D), causal)
+    for name, a, b, t in zip(('o', 'dq', 'dk', 'dv'), run(q, k, v, do, causal=causal), want, tol):
+        step = r * torch.exp2(torch.log2((b.abs() + t).clamp_min(tiny)).floor())
+        off = (a.double() - b).abs() - step - t
+        assert float(off.max()) <= 0, '%s: %.3g of a half step over its tolerance' % (name, float((off / step).max()))
