@@ -6,14 +6,16 @@
 //   dx = rstd (dz w_c - m1 - xhat m2),   m1, m2 = means over the group of dz w_c and dz w_c xhat
 //
 // Both directions are bound by memory.  A sample whose rows fit in the registers of one workgroup is read once and written
-// once (resident kernels; 800 x 196 x 64 fp32: 23 us forward, 30 backward, 3.5 and 4.0 TB/s); a larger one takes a pass for its
-// sums, a small launch that finishes them, and a pass that applies them (16 x 9216 x 320 bf16: 64 us forward, 108 backward, 4.4
-// TB/s over what the passes move).  A thread's sums are per channel, so a group may end anywhere in its vector.
+// once (resident kernels; 800 x 196 x 64 fp32: 23 us forward, 31 backward, 3.5 and 3.9 TB/s; in 16 bits 19 and 25 for half
+// the bytes, so what a value takes besides them shows); a larger one takes a pass for its sums, a small launch that finishes
+// them, and a pass that applies them (16 x 9216 x 320 bf16: 60 us forward, 108 backward, 4.7 and 4.4 TB/s over what the passes
+// move).  A thread's sums are per channel, so a group may end anywhere in its vector.
 //
 // The forward's sums are of d and d^2 in fp64, d = x - (the group's first value): no second pass, and what the variance loses to
 // the mean is 2^-53 of the square of a difference, not of a value.  (Sums of x and x^2 leave 2^-52 x^2 where a group holds
-// one value: at x = 10^5 more than eps, and rstd a third of what it is.  The difference costs the resident forward 4 %.)  The mean is kept as two fp32 numbers for the same
-// reason.  The backward's sums are of mixed sign and fp32 in a thread, fp64 where threads meet.
+// one value: at x = 10^5 more than eps, and rstd a third of what it is.  The difference costs the resident forward 4 %.)  The
+// mean is kept as two fp32 numbers for the same reason.  The backward's sums are of mixed sign and fp32 in a thread, fp64 where
+// threads meet.
 // Sums are added in a fixed order: every run gives the same bits.
 #include "common.h"
 

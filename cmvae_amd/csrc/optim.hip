@@ -9,7 +9,7 @@
 //
 // Bound by memory.  States in 32 bits beside bf16 parameters (22 bytes a value): 123 M values of 44 tensors in 505 us, 5.4 TB/s;
 // 1.1 M fp32 values of 58 tensors in 8 us.  States in 8 bits beside fp32 (16 bytes a value): 98.8 M values in 327 us, 4.8 TB/s;
-// what they stand for, as fp32: 150 us, 6.6 TB/s.
+// what they stand for, as fp32: 156 us, 6.3 TB/s.
 //
 // 8-bit states: 256 consecutive values of a tensor share one fp32 scale per moment.
 //   m: OCP e4m3 of m / s, s = max|m| / 448, to nearest, ties to even;
@@ -18,7 +18,8 @@
 //      its root).  31 octaves below the block's largest, and a root to 3 %, where e4m3 would hold 18.
 //   A moment beyond fp32 (its gradient was not finite, or its square is not) becomes e4m3's NaN / code 255, read as
 //   infinity, and stays out of its block's scale: its neighbours keep theirs.
-// The step itself uses the moments before they are rounded.  Moments and the choice between two neighbouring codes are
+// The step itself uses the moments before they are rounded, in fp32: its few roundings, 2^-24 of the step each, are far under
+// the parameter's own, and a root and a reciprocal in fp64 are not.  Moments and the choice between two neighbouring codes are
 // computed in fp64, which costs no more than fp32 here (the card does 128 fp64 operations per cycle and compute unit, and
 // the kernel waits for memory): a code is then the nearest one of the exact moment, not of a rounded one.
 #include "common.h"
@@ -30,7 +31,7 @@ namespace cmvae {
 namespace opt {
 
 constexpr int PIECE = 4096, BLOCK = 256;        // values per workgroup; values per scale
-constexpr int MAX_T = 96;                       // tensors per launch: 3.6 KB of arguments
+constexpr int MAX_T = 96;                       // tensors per launch: 3.2 KB of arguments
 
 struct Table {
     void* p[MAX_T];

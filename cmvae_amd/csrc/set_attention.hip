@@ -1406,11 +1406,11 @@ static double cost(const Problem& x, const Plan& p) {
 // walk may be cut into pieces, which a second launch joins.
 //   Where four tiles per workgroup fill the card: those, with pieces until there is a workgroup for every slot — twice that for
 // the causal order at one workgroup per unit (two are dealt in pairs, see place()), half again as much where lengths will leave
-// some without work — or, without lengths, whole, if that costs less (20 x 500 rows x 4 heads of 64 bf16, forward: 18 us whole, 27 in
-// two; 8 x 512 against 2048 rows x 8 heads: 48, 36).
+// some without work — or, without lengths, whole, if that costs less (20 x 500 rows x 4 heads of 64 bf16, forward: 23 us whole, 31 in
+// two; 8 x 512 against 2048 rows x 8 heads: 59, 51).
 //   Else whatever costs least of both kinds, whole or in as many pieces as one, two or three turns of the card hold.  Forward +
 //   backward in us, four tiles against one: fp32 4 x 200 rows x 4 heads of 64 67 / 43, 16 x 300 106 / 146, 400 against 8000
-//   141 / 270, causal 4096 x 2 heads of 128 416 / 1261; bf16 32 / 24, 39 / 55, 65 / 78, 160 / 206.
+//   141 / 270, causal 4096 x 2 heads of 128 416 / 1261; bf16 35 / 25, 44 / 59, 74 / 78, 160 / 213.
 static Plan make_plan(const Problem& x) {
     const long cus = compute_units();
     Plan best = plan_with(x, 4, 1);
