@@ -27,7 +27,7 @@ def set_attention(q, k, v, scale=None, causal=False, q_len=None, k_len=None, res
     Probabilities are fp32 and carry a relative error of 2^-24 of their row's largest score; in 16-bit types they, and the scores'
     gradients, are factors of twice the type's bits, so that results are off by their own rounding.  A key that is NaN or infinite
     may reach any row of its batch entry, also those that the causal order hides it from; an infinite value makes NaN.  Scores
-    beyond 2^22 are out of range in float16."""
+    beyond 2^22 are out of range in float16, beyond 2^30 in the other types."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None and q.shape[-1] else scale
     if ops.CHECK_INDICES:
         for t, n, x in ((q_len, 'q_len', q), (k_len, 'k_len', k)):
