@@ -168,11 +168,11 @@ __device__ __forceinline__ f32x16 mul_rows(const char* tile, int row0, const Fra
 // one instruction's eight; the matching first factor — four rows at one channel, twice — comes from the transposing LDS
 // read (16 lanes name 4 rows x 16 channels, lane i receives channel i of the four rows).
 //   16-bit types: the accumulator is a factor twice, as its rounding and as what that leaves.  Every result's error (2-norm,
-// against float64) is then that of its own rounding, to three digits; with one factor o's was 1.16 to 1.31 times that, dq's 1.5 and
-// dk's and dv's 1.42.  One factor (two for dq alone) against two, us: forward + backward of 2 x 4096 causal rows x 16 heads of 128 bf16
-// 870 / 1005, of 8 x 777 against 2049 x 8 heads of 64 fp16 168 / 190; forward of one token x 32 heads of 128 against 16 lists of up
-// to 8191 75.5 / 78.5; dense 8 x 4096 x 16 heads bf16, forward 805 / 1060 (heads of 64) and 1524 / 1790 (128), dk dv 1500 / 1990 and
-// 3720 / 4500.
+// against float64) is then that of its own rounding, to three digits (fp16's dq and dk within 4 %); with one factor o's was 1.16
+// to 1.31 times that, dq's 1.5 and dk's and dv's 1.42.  One factor (two for dq alone) against two, us: forward + backward of 2 x
+// 4096 causal rows x 16 heads of 128 bf16 870 / 1005, of 8 x 777 against 2049 x 8 heads of 64 fp16 168 / 190; forward of one token
+// x 32 heads of 128 against 16 lists of up to 8191 75.5 / 78.5; dense 8 x 4096 x 16 heads bf16, forward 805 / 1060 (heads of 64)
+// and 1524 / 1790 (128), dk dv 1500 / 1990 and 3720 / 4500.
 template <typename T, int D, int ROWS>
 __device__ __forceinline__ void mul_cols(const char* tile, int row0, const f32x16& w, const Sel& sel, f32x16 (&acc)[D / 32]) {
     constexpr int P = Elem<T>::P;
@@ -526,9 +526,9 @@ __device__ __forceinline__ void take_over(const char* smem, int w, float f, f32x
 // Keys in tiles of KT through LDS.  Running maximum m (log2 units) and sum l per row.  nsplit > 1: a workgroup covers one
 // piece of the tiles and leaves (acc, m, l) for the joining kernel.
 //   Bound by the matrix instructions and, between them, the exponentials and the LDS reads that feed them: with two workgroups
-// per unit one computes while the other waits.  Dense 8 x 4096 x 16 heads, bf16: 520 TFLOP/s with 64 channels, 610 with 128 (a
-// large library product reaches 1130), P's second part, half as much again, not counted; fp32 (six bf16 products each), 8 x 2048 x 8 heads: 173 and 150 (the library's fp32
-// product 153).
+// per unit one computes while the other waits.  Dense 8 x 4096 x 16 heads, bf16: 520 TFLOP/s with 64 channels, 610 with 128, P's
+// second part, half as much again, not counted (a large library product reaches 1390); fp32 (six bf16 products each), 8 x 2048 x
+// 8 heads: 173 and 150 (the library's fp32 product 153).
 template <typename T, int D, int NW, int KT, int WS>
 __global__ __launch_bounds__(NW * WS * 64, NW == 4 && sizeof(T) * D <= 256 ? 2 : 1) void fwd_kernel(Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -725,7 +725,7 @@ __device__ __forceinline__ float dot2(unsigned a, unsigned b, float c, _Float16)
 }
 // two values as their roundings and as what those leave
 template <typename T>
-__device__ __forceinline__ void split2(float x, float y, unsigned (&p)[2]) {
+__device__ __forceinline__ void two_parts(float x, float y, unsigned (&p)[2]) {
     typedef T T2 __attribute__((ext_vector_type(2)));
     const T2 a = __builtin_convertvector(f32x2{x, y}, T2);
     p[0] = __builtin_bit_cast(unsigned, a);
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(256) void fwd_rows_kernel(Args a) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     unsigned pp[2];                                 // as in mul_cols(): p's rounding and what that leaves
-                    split2<T>(p[r][u], p[r][u + 1], pp);
+                    two_parts<T>(p[r][u], p[r][u + 1], pp);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) acc[r][e] = dot2(pp[0], y[e], dot2(pp[1], y[e], acc[r][e], T()), T());
                 }
@@ -1446,8 +1446,8 @@ static Plan make_plan(const Problem& x) {
 
 // Rows per key head up to which fwd_rows_kernel takes a list: its arithmetic grows with the rows, the matrix instructions' does
 // not.  Rows kernel / the other, us, for 16 lists of 8191 keys x 8 heads: bf16 heads of 128, 1 row 99 / 102, 2 102 / 104, 4 110 /
-// 101, 8 167 / 105; fp16 heads of 64 50 / 51, 51 / 50, 55 / 50, 102 / 51; fp32 heads of 64, 4 rows 108 / 107 and for 16 of 2000 30 / 34 (6 rows 58 / 35); fp32 heads of 128, 1 row 193 /
-// 332, 8 262 / 330; one list of 8192 keys x 8 heads of 128, 1 row, bf16 10 / 14.
+// 101, 8 167 / 105; fp16 heads of 64 50 / 51, 51 / 50, 55 / 50, 102 / 51; fp32 heads of 64, 4 rows 108 / 107 and for 16 of 2000
+// 30 / 34 (6 rows 58 / 35); fp32 heads of 128, 1 row 193 / 332, 8 262 / 330; one list of 8192 keys x 8 heads of 128, 1 row, bf16 10 / 14.
 constexpr int most_rows(int esize, int D) { return esize == 2 ? 2 : D == 64 ? 4 : 8; }
 
 // Few rows: four waves per workgroup, at least two rounds of 16-byte loads each per piece, eight workgroups per unit (of padded
